@@ -19,6 +19,9 @@
  *                                                                            mg_paged_decode_attn_kv8
  *   transformers sdpa_attention_forward    decode SDPA over the cache        -> mg_paged_decode_attn
  *   microgen/backends/pytorch.py:153-155   greedy torch.argmax               -> mg_argmax_rows
+ *   microgen/backends/pytorch.py:90-116    prompt forward, ragged batches    -> mg_ragged_plan +
+ *                                                                            mg_norm_rope_kv_append + mg_ragged_attn
+ *   microgen/scheduler/speculative.py:21-171 rejection sampling of drafts    -> mg_verify_drafts
  */
 #ifndef MICROGEN_B200_H
 #define MICROGEN_B200_H
@@ -268,6 +271,78 @@ int mg_paged_decode_attn_noalloc(const float* q, const void* k_pool, const void*
                                  const int32_t* block_tables, int max_blocks, const int32_t* ctx_lens, int b,
                                  int hq, int hkv, int d, int n_shared_blocks, float scale, void* out,
                                  void* stream);
+
+/* ---- ragged batches: one step over requests with any number of new tokens each ----------------------
+ * A step of request i brings q_lens[i] >= 0 new tokens on top of ctx_lens[i] >= 0 cached ones: whole prompts
+ * (ctx 0), prompt chunks, single decoding tokens and drafted tokens to verify, in one batch, the new tokens of
+ * all requests packed into rows [cu[i], cu[i+1]). mg_ragged_plan turns the lengths into what the other kernels
+ * of the step read; mg_norm_rope_kv_append and mg_ragged_attn run once per layer on the same plan;
+ * mg_verify_drafts ends a step that verified drafts. Reference counterparts: KVCacheState.update and the
+ * causal SDPA of a prompt forward (kv_cache.py:76-127, pytorch.py:90-116), the target pass and
+ * rejection_sample_token of SpeculativeEngine (scheduler/speculative.py:21-171).
+ *
+ * mg_ragged_plan. In: q_lens, ctx_lens int32 [b]; block_tables int32 [b, max_blocks]; optionally a device free
+ * list: free_blocks int32 [n_free], of which cursor[0] (NULL = 0) are already taken, and held_blocks int32 [b]
+ * (NULL = ceil(ctx / 16)), the blocks each table already holds, which may be more than it needs (a request that
+ * rolled back). Without free_blocks the tables must already hold every block. Out:
+ *   cu_rows int32 [b + 1], kv_lens int32 [b] = ctx + q, per row (max_rows of each) positions, slots (pool slot
+ *   of the row's K/V) and seq_ids; rows behind the last request get position 0, slot -1, seq -1;
+ *   block_tables: request i's missing entries, taken from the free list in request order;
+ *   held_out int32 [b], cursor_out int32 [1]: blocks held and list entries taken after the step;
+ *   work: mg_ragged_plan_bytes() bytes, 16-byte aligned: the attention's work list for hq / hkv heads of d.
+ * The outputs may alias the inputs of the same kind (ctx_lens and kv_lens too). A negative or too long
+ * length, more rows than max_rows, more tokens than max_blocks * 16, or too few free blocks make the plan EMPTY
+ * (cu, kv_lens zero, slots -1, tables, held blocks and cursor as they were) and record MG_ERR_DEVICE (sites
+ * 500..504); a block id outside [0, num_blocks) leaves its rows' slots at -1 (site 505). b <= 8192. */
+int mg_ragged_plan_bytes(int64_t max_rows, int b, int hq, int hkv, int d, size_t* bytes);
+int mg_ragged_plan(const int32_t* q_lens, const int32_t* ctx_lens, int b, int64_t max_rows, int32_t* block_tables,
+                   int max_blocks, int64_t num_blocks, const int32_t* held_blocks, const int32_t* free_blocks,
+                   int64_t n_free, const int32_t* cursor, int hq, int hkv, int d, int32_t* cu_rows,
+                   int32_t* kv_lens, int32_t* positions, int32_t* slots, int32_t* seq_ids, int32_t* held_out,
+                   int32_t* cursor_out, void* work, size_t work_bytes, void* stream);
+/* Per-head norms of q and k, rotary positions and the paged K/V append of `rows` QKV rows. qkv: fp32, or bf16 with
+ * qkv_bf16 != 0, [rows, (hq + 2*hkv) * d], row stride ld_qkv (a multiple of 4 elements), 16-byte aligned.
+ * q_weight / k_weight fp32 [d] (NULL = no norm): y = x * rsqrt(mean(x^2) + eps) * weight over each head; cos_sin as
+ * for mg_rope_kv_append (NULL = no rotation); q_out [rows, hq, d] in bf16 (q_bf16 != 0) or fp32. K and V go to
+ * slots[i] of the pools: bf16, or with k_scales / v_scales int8 codes and scales as mg_rope_kv_append_kv8 stores
+ * them. A row with a negative slot is padding: nothing of it is read or written. A position outside the table
+ * (site 210) or a slot outside the pool (site 211) is recorded and not written. d in {32, 64, 128}. */
+int mg_norm_rope_kv_append(const void* qkv, int qkv_bf16, int64_t ld_qkv, int64_t rows, const int32_t* positions,
+                           const float* cos_sin, int max_pos, const int32_t* slots, const float* q_weight,
+                           const float* k_weight, float eps, int hq, int hkv, int d, void* q_out, int q_bf16,
+                           void* k_pool, void* v_pool, float* k_scales, float* v_scales, int64_t num_blocks,
+                           void* stream);
+/* Causal attention of the planned rows: out bf16 [rows, hq*d]; row r of request i attends to keys 0 .. position(r)
+ * of its block table, whose K/V the step has already appended. q bf16 [rows, hq, d]; pools as for
+ * mg_paged_decode_attn (bf16), or _kv8 (int8) when k_scales / v_scales are given; scale > 0; hq/hkv <= 16;
+ * b, max_rows, hq, hkv, d, block_tables, max_blocks as given to the mg_ragged_plan call that filled `work`.
+ * rows: at least the plan's; rows behind the last request are left as they were. Keys that a row may not see
+ * and pool entries behind a request's last token do not affect it, whatever they hold. workspace: device
+ * scratch of mg_ragged_attn_workspace_bytes() bytes, 16-byte aligned, contents irrelevant: calls that overlap on
+ * the GPU need separate ones. Results do not depend on timing. A plan for other sizes (site 510) or a block id
+ * outside the pool (site 511) is recorded; nothing outside the arrays is read. */
+int mg_ragged_attn_workspace_bytes(int64_t max_rows, int b, int hq, int hkv, int d, size_t* bytes);
+int mg_ragged_attn(const void* q, int64_t rows, const void* k_pool, const void* v_pool, const float* k_scales,
+                   const float* v_scales, int64_t num_blocks, const int32_t* block_tables, int max_blocks, int b,
+                   int64_t max_rows, int hq, int hkv, int d, float scale, const void* work, void* out,
+                   void* workspace, size_t workspace_bytes, void* stream);
+/* Verification of drafted tokens. logits fp32 [rows, vocab] (row stride ld): request i owns rows
+ * cu_rows[i] .. cu_rows[i+1]-1, one after its last accepted token and one after each draft; tokens int32 [rows] are
+ * the tokens that were fed, so the draft which row r asks about is tokens[r + 1]. With p = softmax(logits / T)
+ * (temperatures fp32 [b], NULL = 1) and q the draft's probabilities (draft_probs fp32 [rows, vocab], row r for the
+ * draft asked about at r; NULL = the draft was certain), drafts are accepted in order while u_r q(d) < p(d), u =
+ * uniforms fp32 [rows] in [0, 1); next[i] is then drawn from max(p - q, 0) of the row that stopped (from p behind the
+ * last draft, and where the difference is zero everywhere): the first index whose running sum exceeds
+ * u * total, u = the request's last uniform. T = 0: a draft is accepted iff it is the row's first maximal index
+ * (NaN counting as the maximum), which is also the next token. accepted int32 [b], next int32 [b]. A request
+ * without rows gets (0, -1). Recorded as MG_ERR_DEVICE: cu_rows outside the rows (601) or T < 0 (602), a row without
+ * a softmax (a NaN or +inf logit, or all -inf; 604): next = -1; a drafted token outside the vocabulary (603), which
+ * counts as rejected. workspace: mg_verify_workspace_bytes(), 16-byte aligned. */
+int mg_verify_workspace_bytes(int64_t rows, int64_t vocab, size_t* bytes);
+int mg_verify_drafts(const float* logits, int64_t ld, int64_t rows, int64_t vocab, const int32_t* tokens,
+                     const int32_t* cu_rows, int b, const float* draft_probs, int64_t ld_probs,
+                     const float* uniforms, const float* temperatures, int32_t* accepted, int32_t* next,
+                     void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---- small fused ops of the decode step ---------------------------------------------------- */
 /* h fp32 [b, hidden] = wte[tokens[i]] (+ wpe[positions[i]] when wpe != NULL). */

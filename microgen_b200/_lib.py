@@ -55,6 +55,15 @@ SIGNATURES = {
     "mg_paged_decode_attn": [_p, _p, _p, _i64, _p, _i, _p, _i, _i, _i, _i, _i, _f, _p, _p, _sz, _p],
     "mg_paged_decode_attn_kv8": [_p, _p, _p, _p, _p, _i64, _p, _i, _p, _i, _i, _i, _i, _i, _f, _p, _p, _sz, _p],
     "mg_paged_decode_attn_noalloc": [_p, _p, _p, _i64, _p, _i, _p, _i, _i, _i, _i, _i, _f, _p, _p],
+    "mg_ragged_plan_bytes": [_i64, _i, _i, _i, _i, C.POINTER(C.c_size_t)],
+    "mg_ragged_plan": [_p, _p, _i, _i64, _p, _i, _i64, _p, _p, _i64, _p, _i, _i, _i, _p, _p, _p, _p, _p, _p, _p, _p,
+                       _sz, _p],
+    "mg_norm_rope_kv_append": [_p, _i, _i64, _i64, _p, _p, _i, _p, _p, _p, _f, _i, _i, _i, _p, _i, _p, _p, _p, _p,
+                               _i64, _p],
+    "mg_ragged_attn_workspace_bytes": [_i64, _i, _i, _i, _i, C.POINTER(C.c_size_t)],
+    "mg_ragged_attn": [_p, _i64, _p, _p, _p, _p, _i64, _p, _i, _i, _i64, _i, _i, _i, _f, _p, _p, _p, _sz, _p],
+    "mg_verify_workspace_bytes": [_i64, _i64, C.POINTER(C.c_size_t)],
+    "mg_verify_drafts": [_p, _i64, _i64, _i64, _p, _p, _i, _p, _i64, _p, _p, _p, _p, _p, _sz, _p],
     "mg_embed": [_p, _p, _p, _p, _i, _i, _i64, _i, _p, _p],
     "mg_rmsnorm": [_p, _p, _i, _i, _f, _p, _p],
     "mg_layernorm": [_p, _p, _p, _i, _i, _f, _p, _p],
@@ -76,7 +85,8 @@ LAUNCHING = {"mg_quantize_rows_i8", "mg_i8_linear", "mg_i8_linear_simt", "mg_i8_
              "mg_i8_linear_packed_rowpar_sk",
              "mg_paged_decode_attn", "mg_embed", "mg_rmsnorm", "mg_layernorm", "mg_argmax_rows",
              "mg_decode_advance", "mg_decode_block", "mg_vocab_argmax", "mg_rope_kv_append_kv8",
-             "mg_paged_decode_attn_kv8"}
+             "mg_paged_decode_attn_kv8", "mg_ragged_plan", "mg_norm_rope_kv_append", "mg_ragged_attn",
+             "mg_verify_drafts"}
 LAUNCHES = [0]  # kernels launched (or captured) through call() in this process
 
 _lock = threading.Lock()

@@ -218,6 +218,244 @@ def paged_decode_attn(q, k_pool, v_pool, block_tables, ctx_lens, scale, n_shared
     return out
 
 
+# ---- ragged batches: any number of new tokens per request --------------------------------------------
+class RaggedPlan:
+    """Device buffers of one step over ``b`` requests with up to ``max_rows`` new tokens in all, block tables of
+    ``max_blocks`` entries and attention over ``hq`` / ``hkv`` heads of ``d``: filled by ``ragged_plan``, read by
+    ``ragged_attn`` of every layer. One plan serves a stream-ordered sequence of steps; steps that overlap on the GPU
+    (two streams, two graphs replayed at once) need a plan each, because it also holds the attention's workspace.
+
+    ``cu_rows`` int32 [b+1], ``kv_lens`` int32 [b], ``positions`` / ``slots`` / ``seq_ids`` int32 [max_rows],
+    ``n_blocks`` int32 [b] and ``cursor`` int32 [1] (blocks held and free-list entries taken after the step)."""
+
+    def __init__(self, b: int, max_rows: int, max_blocks: int, hq: int, hkv: int, d: int, device) -> None:
+        self.b, self.max_rows, self.max_blocks = int(b), int(max_rows), int(max_blocks)
+        self.hq, self.hkv, self.d, self.device = int(hq), int(hkv), int(d), torch.device(device)
+        if self.device.type != "cuda":
+            raise ValueError("a plan lives on a CUDA device (the ragged path has no CPU fallback)")
+        if self.device.index is None:
+            self.device = torch.device("cuda", torch.cuda.current_device())
+        if self.max_blocks < 1:
+            raise ValueError("max_blocks must be at least 1")
+        n, ws = C.c_size_t(0), C.c_size_t(0)
+        with torch.cuda.device(self.device):
+            _lib.call("mg_ragged_plan_bytes", self.max_rows, self.b, self.hq, self.hkv, self.d, C.byref(n))
+            _lib.call("mg_ragged_attn_workspace_bytes", self.max_rows, self.b, self.hq, self.hkv, self.d, C.byref(ws))
+        i32 = dict(dtype=torch.int32, device=self.device)
+        self.cu_rows = torch.zeros(self.b + 1, **i32)
+        self.kv_lens, self.n_blocks = torch.zeros(self.b, **i32), torch.zeros(self.b, **i32)
+        self.positions, self.slots, self.seq_ids = (torch.zeros(self.max_rows, **i32) for _ in range(3))
+        self.cursor = torch.zeros(1, **i32)
+        self.work = torch.zeros(n.value, dtype=torch.uint8, device=self.device)
+        self.workspace = torch.empty(ws.value, dtype=torch.uint8, device=self.device)
+        self.tables: torch.Tensor | None = None
+
+
+def _on(device, **tensors) -> None:
+    for name, t in tensors.items():
+        if t is not None and t.device != device:
+            raise ValueError(f"{name} is on {t.device}, expected {device}")
+
+
+def _vec_i32(t, n, name: str) -> None:
+    _need(t, torch.int32, name)
+    if t.dim() != 1 or (n is not None and t.shape[0] != n):
+        raise ValueError(f"{name} must be int32 [{n if n is not None else 'n'}], got {tuple(t.shape)}")
+
+
+def ragged_plan(plan: RaggedPlan, q_lens, ctx_lens, tables, num_blocks: int, n_blocks=None, free_blocks=None,
+                cursor=None) -> RaggedPlan:
+    """Plan a step in which request i adds ``q_lens[i]`` tokens to its ``ctx_lens[i]`` cached ones (int32 [b]).
+
+    ``tables`` int32 [b, max_blocks] must hold every block of ctx + q, or a device free list is given:
+    ``free_blocks`` int32 [F] with ``cursor`` int32 [1] of its entries already taken (None = 0) and ``n_blocks``
+    int32 [b] blocks already in each table (None = those of ctx); the missing entries are then written into
+    ``tables``. ``plan.n_blocks`` and ``plan.cursor`` hold the counts after the step and may be passed back in (as
+    may ``plan.kv_lens`` for ctx_lens). Impossible lengths or an exhausted list make an empty plan, and
+    ``check_device`` raises."""
+    _vec_i32(q_lens, plan.b, "q_lens")
+    _vec_i32(ctx_lens, plan.b, "ctx_lens")
+    _need(tables, torch.int32, "tables")
+    if tables.shape != (plan.b, plan.max_blocks):
+        raise ValueError(f"tables must be [{plan.b}, {plan.max_blocks}], got {tuple(tables.shape)}")
+    if n_blocks is not None:
+        _vec_i32(n_blocks, plan.b, "n_blocks")
+    if free_blocks is not None:
+        _vec_i32(free_blocks, None, "free_blocks")
+    if cursor is not None:
+        if free_blocks is None:
+            raise ValueError("a cursor needs the free list it counts in")
+        _vec_i32(cursor, 1, "cursor")
+    _on(plan.device, q_lens=q_lens, ctx_lens=ctx_lens, tables=tables, n_blocks=n_blocks, free_blocks=free_blocks,
+        cursor=cursor)
+    # an empty free list still has an address, so that running out of it is noticed
+    free = free_blocks if free_blocks is None or free_blocks.numel() else plan.cursor
+    with torch.cuda.device(plan.device):
+        _lib.call("mg_ragged_plan", _ptr(q_lens), _ptr(ctx_lens), plan.b, plan.max_rows, _ptr(tables), plan.max_blocks,
+                  int(num_blocks), _ptr(n_blocks), _ptr(free), 0 if free_blocks is None else free_blocks.numel(),
+                  _ptr(cursor), plan.hq, plan.hkv, plan.d, _ptr(plan.cu_rows), _ptr(plan.kv_lens),
+                  _ptr(plan.positions), _ptr(plan.slots), _ptr(plan.seq_ids), _ptr(plan.n_blocks), _ptr(plan.cursor),
+                  _ptr(plan.work), plan.work.numel(), _stream())
+    plan.tables = tables
+    return plan
+
+
+def _pools(k_pool, v_pool, k_scales, v_scales, hkv: int, d: int) -> bool:
+    """Check a K/V pool pair (and its scales when int8); True for int8."""
+    q8 = k_pool.dtype == torch.int8
+    dt = torch.int8 if q8 else torch.bfloat16
+    _need(k_pool, dt, "k_pool")
+    _need(v_pool, dt, "v_pool")
+    want = (k_pool.shape[0], hkv, BLOCK_SIZE, d)
+    if tuple(k_pool.shape) != want or tuple(v_pool.shape) != want or want[0] < 1:
+        raise ValueError(f"pools must be [num_blocks, {hkv}, {BLOCK_SIZE}, {d}], got {tuple(k_pool.shape)} and "
+                         f"{tuple(v_pool.shape)}")
+    if not q8 and (k_scales is not None or v_scales is not None):
+        raise ValueError("scales belong to int8 pools")
+    if q8:
+        for t, name in ((k_scales, "k_scales"), (v_scales, "v_scales")):
+            if t is None:
+                raise ValueError(f"int8 pools need {name}")
+            _need(t, torch.float32, name)
+            if tuple(t.shape) != want[:3]:
+                raise ValueError(f"{name} must be {list(want[:3])}, got {tuple(t.shape)}")
+    return q8
+
+
+def norm_rope_kv_append(qkv, positions, cos_sin, slots, hq, hkv, d, k_pool, v_pool, q_weight=None, k_weight=None,
+                        eps: float = 1e-6, q_out=None, k_scales=None, v_scales=None):
+    """Per-head RMS norms of q and k (where a weight fp32 [d] is given), RoPE (where a table is given) and the paged
+    K/V append of every row of ``qkv`` (fp32 or bf16 [rows, (hq+2*hkv)*d], unit inner stride). Returns q bf16
+    [rows, hq, d] (or ``q_out``, bf16 or fp32). int8 pools store each K and V vector quantized with its scale. Rows
+    whose slot is negative are padding and left alone: with padding rows pass ``q_out``, whose rows then stay."""
+    if not qkv.is_cuda or qkv.dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError("qkv must be a CUDA tensor, fp32 or bf16 (the ragged path has no CPU fallback)")
+    rows = qkv.shape[0]
+    if qkv.dim() != 2 or qkv.shape[1] != (hq + 2 * hkv) * d or qkv.stride(1) != 1:
+        raise ValueError(f"qkv must be [rows, {(hq + 2 * hkv) * d}] with unit inner stride, got {tuple(qkv.shape)}")
+    ld = qkv.stride(0) if rows > 1 else qkv.shape[1]
+    if ld < qkv.shape[1] or ld % 4:
+        raise ValueError("rows of qkv must not overlap, and start a multiple of 4 elements apart")
+    _vec_i32(slots, rows, "slots")
+    if cos_sin is not None:
+        _need(cos_sin, torch.float32, "cos_sin")
+        if cos_sin.dim() != 2 or cos_sin.shape[1] != d:
+            raise ValueError(f"cos_sin must be [max_pos, {d}]")
+        _vec_i32(positions, rows, "positions")
+    for t, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
+        if t is not None:
+            _need(t, torch.float32, name)
+            if tuple(t.shape) != (d,):
+                raise ValueError(f"{name} must be [{d}]")
+    _pools(k_pool, v_pool, k_scales, v_scales, hkv, d)
+    if q_out is None:
+        q_out = torch.empty((rows, hq, d), dtype=torch.bfloat16, device=qkv.device)
+    if q_out.dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError("q_out must be bf16 or fp32")
+    _need(q_out, q_out.dtype, "q_out")
+    if q_out.numel() != rows * hq * d:
+        raise ValueError(f"q_out must be [{rows}, {hq}, {d}]")
+    _on(qkv.device, positions=positions if cos_sin is not None else None, cos_sin=cos_sin, slots=slots, k_pool=k_pool,
+        v_pool=v_pool, q_weight=q_weight, k_weight=k_weight, q_out=q_out, k_scales=k_scales, v_scales=v_scales)
+    with torch.cuda.device(qkv.device):
+        _lib.call("mg_norm_rope_kv_append", _ptr(qkv), int(qkv.dtype == torch.bfloat16), ld, rows,
+                  _ptr(positions if cos_sin is not None else None), _ptr(cos_sin),
+                  0 if cos_sin is None else cos_sin.shape[0], _ptr(slots), _ptr(q_weight), _ptr(k_weight), float(eps),
+                  hq, hkv, d, _ptr(q_out), int(q_out.dtype == torch.bfloat16), _ptr(k_pool), _ptr(v_pool),
+                  _ptr(k_scales), _ptr(v_scales), k_pool.shape[0], _stream())
+    return q_out
+
+
+def ragged_attn(q, k_pool, v_pool, plan: RaggedPlan, scale, out=None, k_scales=None, v_scales=None):
+    """Causal attention of a planned step (``ragged_plan``) over its paged K/V: q bf16 [rows, hq, d], the plan's rows
+    in order (rows behind them are ignored, and stay as they were in a given ``out``); pools bf16, or int8 with
+    scales. Returns bf16 [rows, hq*d]. The step's own K/V must already be in the pools."""
+    if plan.tables is None:
+        raise ValueError("the plan has not been filled: call ragged_plan first")
+    _need(q, torch.bfloat16, "q")
+    if q.dim() != 3 or tuple(q.shape[1:]) != (plan.hq, plan.d):
+        raise ValueError(f"q must be [rows, {plan.hq}, {plan.d}], got {tuple(q.shape)}")
+    _pools(k_pool, v_pool, k_scales, v_scales, plan.hkv, plan.d)
+    if not float(scale) > 0.0:
+        raise ValueError("scale must be positive")
+    rows = q.shape[0]
+    if out is None:
+        out = torch.empty((rows, plan.hq * plan.d), dtype=torch.bfloat16, device=q.device)
+    _need(out, torch.bfloat16, "out")
+    if out.numel() != rows * plan.hq * plan.d:
+        raise ValueError(f"out must be [{rows}, {plan.hq * plan.d}]")
+    _on(plan.device, q=q, k_pool=k_pool, v_pool=v_pool, out=out, k_scales=k_scales, v_scales=v_scales)
+    with torch.cuda.device(plan.device):
+        _lib.call("mg_ragged_attn", _ptr(q), rows, _ptr(k_pool), _ptr(v_pool), _ptr(k_scales), _ptr(v_scales),
+                  k_pool.shape[0], _ptr(plan.tables), plan.max_blocks, plan.b, plan.max_rows, plan.hq, plan.hkv,
+                  plan.d, float(scale), _ptr(plan.work), _ptr(out), _ptr(plan.workspace), plan.workspace.numel(),
+                  _stream())
+    if rows:
+        _lib.LAUNCHES[0] += 1  # the merge of split items
+    return out
+
+
+def verify_workspace_bytes(rows: int, vocab: int) -> int:
+    n = C.c_size_t(0)
+    _lib.call("mg_verify_workspace_bytes", int(rows), int(vocab), C.byref(n))
+    return int(n.value)
+
+
+def verify_drafts(logits, tokens, cu_rows, uniforms, draft_probs=None, temperatures=None, accepted=None, next_tokens=None,
+                  workspace=None):
+    """Accept drafted tokens by the rejection rule of speculative sampling and draw each request's next token.
+
+    logits fp32 [rows, vocab] (unit inner stride); request i owns rows ``cu_rows[i]`` to ``cu_rows[i+1]`` (int32
+    [b+1]), its last accepted token's and then one per draft; ``tokens`` int32 [rows] are the tokens that were fed
+    (so row r asks about tokens[r+1]); ``uniforms`` fp32 [rows] in [0, 1); ``draft_probs`` fp32 [rows, vocab], the
+    draft's distribution at each asking row (None: the drafts were certain); ``temperatures`` fp32 [b] (None: 1; 0:
+    greedy). Returns (accepted int32 [b], next token int32 [b]); see ``mg_verify_drafts`` for the rule."""
+    _need(logits, torch.float32, "logits", contiguous=False)
+    if logits.dim() != 2 or logits.stride(1) != 1 or logits.shape[1] < 1:
+        raise ValueError("logits must be [rows, vocab] with unit inner stride")
+    rows, vocab = logits.shape
+    ld = logits.stride(0) if rows > 1 else vocab
+    _vec_i32(tokens, rows, "tokens")
+    _vec_i32(cu_rows, None, "cu_rows")
+    b = cu_rows.shape[0] - 1
+    if b < 0:
+        raise ValueError("cu_rows must be int32 [b + 1]")
+    _need(uniforms, torch.float32, "uniforms")
+    if tuple(uniforms.shape) != (rows,):
+        raise ValueError(f"uniforms must be [{rows}]")
+    ldq = vocab
+    if draft_probs is not None:
+        _need(draft_probs, torch.float32, "draft_probs", contiguous=False)
+        if tuple(draft_probs.shape) != (rows, vocab) or draft_probs.stride(1) != 1:
+            raise ValueError(f"draft_probs must be [{rows}, {vocab}] with unit inner stride")
+        ldq = draft_probs.stride(0) if rows > 1 else vocab
+    if ld < vocab or ldq < vocab:
+        raise ValueError("rows of logits and draft_probs must not overlap")
+    if temperatures is not None:
+        _need(temperatures, torch.float32, "temperatures")
+        if tuple(temperatures.shape) != (b,):
+            raise ValueError(f"temperatures must be [{b}]")
+    dev = logits.device
+    if accepted is None:
+        accepted = torch.empty(b, dtype=torch.int32, device=dev)
+    if next_tokens is None:
+        next_tokens = torch.empty(b, dtype=torch.int32, device=dev)
+    _vec_i32(accepted, b, "accepted")
+    _vec_i32(next_tokens, b, "next_tokens")
+    with torch.cuda.device(dev):
+        ws = verify_workspace_bytes(rows, vocab)
+        if workspace is None or workspace.numel() * workspace.element_size() < ws:
+            workspace = torch.empty(ws, dtype=torch.uint8, device=dev)
+        _on(dev, tokens=tokens, cu_rows=cu_rows, uniforms=uniforms, draft_probs=draft_probs, temperatures=temperatures,
+            accepted=accepted, next_tokens=next_tokens, workspace=workspace)
+        _lib.call("mg_verify_drafts", _ptr(logits), ld, rows, vocab, _ptr(tokens), _ptr(cu_rows), b, _ptr(draft_probs),
+                  ldq, _ptr(uniforms), _ptr(temperatures), _ptr(accepted), _ptr(next_tokens), _ptr(workspace), ws,
+                  _stream())
+    if rows and b:
+        _lib.LAUNCHES[0] += 1  # the row statistics, then the decision
+    return accepted, next_tokens
+
+
 def embed(tokens, positions, wte, wpe, h):
     _need(tokens, torch.int32, "tokens")
     _need(wte, torch.float32, "wte")

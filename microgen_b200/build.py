@@ -3,7 +3,7 @@
     python -m microgen_b200.build [--force] [--verbose]
 
 Each ``csrc/*.cu`` is compiled with relocatable device code (the device error
-word is shared across translation units) and linked, device link included,
+word is shared across translation units; ``OWN_MODULE`` lists the exceptions) and linked, device link included,
 into ``microgen_b200/libmicrogen_b200.so`` next to this file. CUDA runtime is
 linked statically; the driver entry point the TMA descriptors need is
 resolved at run time through ``cudaGetDriverEntryPoint``.
@@ -26,6 +26,9 @@ LIB = os.path.join(HERE, "libmicrogen_b200.so")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-rdc=true", "-Xcompiler", "-fPIC,-O2", "--expt-relaxed-constexpr",
          "-Xptxas", "-warn-spills"]
+# Sources compiled as modules of their own: register reallocation between warps (setmaxnreg) is ignored in
+# relocatable device code. They reach the device error words through their launch arguments.
+OWN_MODULE = {"ragged_attn.cu"}
 
 
 def nvcc() -> str:
@@ -62,7 +65,10 @@ def build(force: bool = False, verbose: bool = False, extra: list[str] | None = 
         o = os.path.join(BUILD, os.path.basename(s)[:-3] + ".o")
         objs.append(o)
         if force or _stale(o, [s] + hdrs):
-            cmd = [nvcc()] + ARCH + FLAGS + (extra or []) + ["-I", INCLUDE, "-c", s, "-o", o]
+            flags = FLAGS
+            if os.path.basename(s) in OWN_MODULE:
+                flags = [f for f in FLAGS if f != "-rdc=true"] + ["-DMG_ERROR_WORDS_SHARED"]
+            cmd = [nvcc()] + ARCH + flags + (extra or []) + ["-I", INCLUDE, "-c", s, "-o", o]
             jobs.append(cmd)
 
     def run(cmd):

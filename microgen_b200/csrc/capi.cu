@@ -52,6 +52,36 @@ int mg_make_map_2d(CUtensorMap* map, CUtensorMapDataType dt, const void* base, u
   return r == CUDA_SUCCESS ? MG_OK : MG_ERR_INVALID_ARG;
 }
 
+int mg_make_map_3d(CUtensorMap* map, CUtensorMapDataType dt, const void* base, const uint64_t (&dims)[3],
+                   const uint64_t (&strides)[2], const uint32_t (&box)[3], CUtensorMapSwizzle swizzle) {
+  PFN_encodeTiled_t enc = get_encode_fn();
+  if (!enc) return MG_ERR_CUDA;
+  cuuint64_t d[3] = {dims[0], dims[1], dims[2]}, st[2] = {strides[0], strides[1]};
+  cuuint32_t b[3] = {box[0], box[1], box[2]}, es[3] = {1, 1, 1};
+  CUresult r = enc(map, dt, 3, const_cast<void*>(base), d, st, b, es, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? MG_OK : MG_ERR_INVALID_ARG;
+}
+
+int mg_error_words(int** code, int** info) {
+  static int* addr[64][2] = {};
+  static std::mutex mu;
+  int dev = 0;
+  MG_CUDA_TRY(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 64) return MG_ERR_UNSUPPORTED;
+  std::lock_guard<std::mutex> lock(mu);
+  if (!addr[dev][1]) {
+    void *c = nullptr, *i = nullptr;
+    MG_CUDA_TRY(cudaGetSymbolAddress(&c, g_mg_dev_error));
+    MG_CUDA_TRY(cudaGetSymbolAddress(&i, g_mg_dev_error_info));
+    addr[dev][0] = static_cast<int*>(c);
+    addr[dev][1] = static_cast<int*>(i);
+  }
+  *code = addr[dev][0];
+  *info = addr[dev][1];
+  return MG_OK;
+}
+
 extern "C" int mg_abi_version(void) { return MG_ABI_VERSION; }
 
 extern "C" const char* mg_status_string(int status) {

@@ -18,12 +18,31 @@
 #define MG_SPIN_LIMIT (1u << 22)
 
 // Device-side error word (first error wins). Read by mg_device_error().
+#ifndef MG_ERROR_WORDS_SHARED
 extern __device__ int g_mg_dev_error;
 extern __device__ int g_mg_dev_error_info;
+#endif
 
+#ifdef MG_ERROR_WORDS_SHARED
+// A source compiled as a module of its own (no relocatable device code, see build.py) cannot name the device
+// error words of another module: each of its CTAs keeps their addresses, which the launch passes in, in shared memory
+// (mg_set_error_words, before the first barrier).
+static __shared__ int* s_mg_error[2];
+__device__ __forceinline__ void mg_set_error_words(int* code, int* info) {
+  s_mg_error[0] = code;
+  s_mg_error[1] = info;
+}
+__device__ __forceinline__ void mg_record_error(int code, int info) {
+  if (atomicCAS(s_mg_error[0], 0, code) == 0) *s_mg_error[1] = info;
+}
+#else
 __device__ __forceinline__ void mg_record_error(int code, int info) {
   if (atomicCAS(&g_mg_dev_error, 0, code) == 0) g_mg_dev_error_info = info;
 }
+#endif
+
+// Host: device addresses of the error words on the current device.
+int mg_error_words(int** code, int** info);
 
 // Host-side: remember the last CUDA error for mg_last_cuda_error().
 int mg_set_cuda_error(cudaError_t e);
@@ -68,6 +87,10 @@ inline cudaError_t mg_once_per_device(bool (&flags)[64], std::mutex& mu, F&& set
 // Host: a 2-D tiled TMA descriptor (row-major [outer][inner], row_bytes apart; box_inner x box_outer).
 int mg_make_map_2d(CUtensorMap* map, CUtensorMapDataType dt, const void* base, uint64_t inner, uint64_t outer,
                    uint64_t row_bytes, uint32_t box_inner, uint32_t box_outer, CUtensorMapSwizzle swizzle);
+
+// The same for three dimensions (strides in bytes of the outer two).
+int mg_make_map_3d(CUtensorMap* map, CUtensorMapDataType dt, const void* base, const uint64_t (&dims)[3],
+                   const uint64_t (&strides)[2], const uint32_t (&box)[3], CUtensorMapSwizzle swizzle);
 
 template <typename... KArgs, typename... Args>
 static inline cudaError_t mg_launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st,
@@ -258,6 +281,13 @@ __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, u
       "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(
           smem_u32(dst)),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
+          smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
       : "memory");
 }
 // Untiled bulk copy global -> this CTA's shared memory (no multicast): both addresses 16-byte aligned,

@@ -37,21 +37,32 @@ struct RagCfg {
   static constexpr int kSlabs = D * 2 / kSlab;                     // slabs side by side in a tile
   static constexpr int kSlabBytes = kRows * kSlab;
   static constexpr int kTileBytes = kRows * D * 2;
-  static constexpr int kStages = D == 128 ? (Q8 ? 4 : 5) : (D == 64 ? 8 : 12);
+  static constexpr int kStages = D == 128 ? (Q8 ? 3 : 5) : (D == 64 ? 6 : 8);
+  static constexpr int kCodeStages = Q8 ? (D == 128 ? 3 : 4) : 0;  // int8 codes on their way to a stage
+  static constexpr int kCodeBytes = kRows * D;
   // the scales of a tile are read until its softmax is done, which the stage of K (free once S is) does not wait for:
   // a tile's K may be stored while the kStages / 2 tiles before it are still at work
   static constexpr int kScaleRing = kStages / 2 + 1;
-  static constexpr int kQ = 0;
-  static constexpr int kRing = 2 * kTileBytes;
-  static constexpr int kScales = kRing + kStages * kTileBytes;     // [ring][K 128 | V 128] fp32
-  static constexpr int kBars = kScales + (Q8 ? kScaleRing * 2 * kRows * 4 : 0);
+  static constexpr int kRing = 2 * kTileBytes;                     // (the two tiles of Q come first)
+  static constexpr int kCodes = kRing + kStages * kTileBytes;
+  static constexpr int kCodeScales = kCodes + kCodeStages * kCodeBytes;
+  static constexpr int kScales = kCodeScales + kCodeStages * kRows * 4;  // [ring][K 128 | V 128] fp32
+  static constexpr int kMl = kScales + (Q8 ? kScaleRing * 2 * kRows * 4 : 0);  // [128] (maximum, sum)
+  static constexpr int kBars = kMl + kRows * 8;
   static constexpr int kSmem = kBars + 512 + 1024;
-  static constexpr int kThreads = Q8 ? 13 * 32 : 10 * 32;
+  static_assert(kSmem <= 232448 - 64, "shared memory");
+  static constexpr int kThreads = Q8 ? 512 : 384;
+  // registers: a block of 384 threads starts with 168 each, one of 512 with 128; the warpgroups' shares add up to that
+  static constexpr int kSoftRegs = Q8 ? 184 : 208;
+  static constexpr int kOtherRegs = Q8 ? 72 : 88;
+  static_assert(2 * kSoftRegs + (kThreads / 128 - 2) * kOtherRegs <= (kThreads / 128) * (Q8 ? 128 : 168), "registers");
   static constexpr uint32_t kO = 256;                              // tensor-memory columns: S0, S1, O0, O1
   // fp32 accumulator, bf16 operands, M = 128; S: K-major B of N = 128; O: MN-major B of N = D
   static constexpr uint32_t kIdescS = (1u << 4) | (1u << 7) | (1u << 10) | ((kRows >> 3) << 17) | ((kRows >> 4) << 24);
   static constexpr uint32_t kIdescO =
       (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((kRows >> 4) << 24);
+  // one in kPolyEvery pairs of exponentials is computed on the FMA pipe (0: none)
+  static constexpr int kPolyEvery = 0;
 };
 
 // Byte offset of the 16-byte chunk `c` (8 bf16) of row r in a swizzled tile.
@@ -82,8 +93,101 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+               "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+               : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr),
+               "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr));
+}
+
+// One lane of a converged warp. The compiler knows that elect.sync leaves a single thread, and issues a tensor-core
+// product, a commit or a TMA copy in its branch once; behind `lane == 0` it has to allow for several threads, which
+// measured 91 cycles a product (64 is the hardware's rate) and 60 a commit (7).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.b32 %0, 1, 0, q;\n\t}" : "=r"(p));
+  return p != 0;
+}
+__device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
+
+// mbar_wait with its polls in one asm loop: 43 cycles where the phase is already over, 179 as a C++ loop.
+__device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity, int where) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .u32 n;\n\tmov.u32 n, %3;\n\t"
+      "POLL:\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "@p bra DONE;\n\t"
+      "sub.u32 n, n, 1;\n\tsetp.ne.u32 q, n, 0;\n\t@q bra POLL;\n\t"
+      "DONE:\n\tselp.b32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity), "n"(MG_SPIN_LIMIT)
+      : "memory");
+  if (!ok) mg_record_error(MG_ERR_TIMEOUT, where);
+  return ok != 0;
+}
+
+template <int N>
+__device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
+// Pairs of fp32 in one 64-bit register: one FMA-pipe instruction for two values.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpair(uint64_t p, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// 2^x of a pair, x <= 127, on the FMA pipe: x = n + f with n the nearest integer (adding 1.5 * 2^23 leaves n in the low
+// mantissa bits), 2^f on [-1/2, 1/2] by a degree-4 polynomial fitted for the least relative error (2.7e-6, well
+// below the 2^-9 of rounding P to bf16), and n added to the exponent. Below 2^-126 the result is some tiny number.
+__device__ __forceinline__ uint64_t ex2_poly2(uint64_t x) {
+  float a, b;
+  unpair(x, a, b);
+  x = pair(fmaxf(a, -126.f), fmaxf(b, -126.f));
+  const uint64_t magic = pair(12582912.f, 12582912.f), minus = pair(-12582912.f, -12582912.f);
+  const uint64_t t = add2(x, magic);
+  const uint64_t f = fma2(add2(t, minus), pair(-1.f, -1.f), x);
+  uint64_t y = fma2(pair(0.009570100344717503f, 0.009570100344717503f), f, pair(0.05591785907745361f, 0.05591785907745361f));
+  y = fma2(y, f, pair(0.240247443318367f, 0.240247443318367f));
+  y = fma2(y, f, pair(0.6931217908859253f, 0.6931217908859253f));
+  y = fma2(y, f, pair(0.9999992847442627f, 0.9999992847442627f));
+  float ta, tb, ya, yb;
+  unpair(t, ta, tb);
+  unpair(y, ya, yb);
+  return pair(__int_as_float(__float_as_int(ya) + (__float_as_int(ta) << 23)),
+              __int_as_float(__float_as_int(yb) + (__float_as_int(tb) << 23)));
+}
+
 struct RagArgs {
-  const __nv_bfloat16* q;
   int64_t rows, num_blocks;
   const int32_t* tables;
   int max_blocks, b, hq, hkv, group, tok_tile, max_slots;
@@ -95,63 +199,111 @@ struct RagArgs {
   __nv_bfloat16* out;
   float* ws_o;   // [slots][hkv][2 * 128][D]
   float2* ws_ml; // [slots][hkv][2 * 128]: maximum in log2 units, sum
+  int *err_code, *err_info;
 };
+
+// A CTA's k-th piece of work: an entry of the list and a K/V head. The list is sorted, longest first, and dealt out
+// forwards and backwards in turn, which evens out the CTAs' sums.
+struct RagWork {
+  RagItem it;
+  int head, tiles;    // K/V head; K/V tiles of the item
+  int n0, n1;         // K/V tiles that each softmax warpgroup visits
+  bool dual;          // one row tile: the warpgroups take its K/V tiles in turn
+};
+
+__device__ __forceinline__ int rag_index(int k, int total) {
+  const int g = (int)gridDim.x, c = (int)blockIdx.x;
+  const int64_t i = (int64_t)k * g + (k & 1 ? g - 1 - c : c);
+  return i < total ? (int)i : -1;
+}
+__device__ __forceinline__ RagItem rag_item(const RagArgs& p, int index) {
+  RagItem r = {};
+  if (index >= 0) {
+    const int4* src = reinterpret_cast<const int4*>(p.work + p.list_off) + 2 * (index / p.hkv);
+    const int4 a = __ldg(src), b = __ldg(src + 1);
+    r.seq = a.x, r.row0 = a.y, r.n_tok = a.z, r.pos0 = a.w;
+    r.kt0 = b.x, r.kt1 = b.y, r.slot = b.z, r.kv_len = b.w;
+  }
+  return r;
+}
+// The work of an item; one that does not fit this call's arrays (a plan for other sizes) has no tiles.
+__device__ __forceinline__ RagWork rag_work(const RagArgs& p, const RagItem& it, int index) {
+  RagWork w;
+  w.it = it;
+  w.head = index % p.hkv;
+  const bool fits = it.row0 >= 0 && it.n_tok > 0 && (int64_t)it.row0 + it.n_tok <= p.rows && it.seq >= 0 && it.seq < p.b &&
+                    it.kt0 >= 0 && it.kt1 > it.kt0 && (int64_t)it.kv_len <= (int64_t)p.max_blocks * 16 &&
+                    (int64_t)(it.kt1 - 1) * kRows < it.kv_len && it.slot < p.max_slots;
+  if (!fits) {
+    w.it.n_tok = 0;
+    w.n0 = w.n1 = w.tiles = 0;
+    w.dual = false;
+    return w;
+  }
+  const int tiles = it.kt1 - it.kt0;
+  w.dual = it.n_tok <= p.tok_tile;
+  if (w.dual) {
+    w.n0 = (tiles + 1) >> 1;
+    w.n1 = tiles >> 1;
+    w.tiles = tiles;
+  } else {  // the first row tile ends at its own last token
+    const int last = it.pos0 + p.tok_tile - 1;
+    w.n0 = max(0, min(it.kt1, last / kRows + 1) - it.kt0);
+    w.n1 = tiles;
+    w.tiles = tiles;
+  }
+  return w;
+}
 
 template <int D, bool Q8>
 __global__ void __launch_bounds__(RagCfg<D, Q8>::kThreads, 1)
-    ragged_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
-                       const RagArgs p) {
+    ragged_attn_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
+                       const __grid_constant__ CUtensorMap tv, const RagArgs p) {
   using C = RagCfg<D, Q8>;
   constexpr int NS = C::kStages;
+  constexpr int NC = C::kCodeStages > 0 ? C::kCodeStages : 1;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kBars);
   uint64_t* empty = full + NS;
-  uint64_t* sfull = empty + NS;    // [2] a row tile's scores are in tensor memory (and its earlier P V is done)
-  uint64_t* pready = sfull + 2;    // [2] its probabilities are
-  uint64_t* ofull = pready + 2;    // [2] its output is complete
-  uint64_t* qfull = ofull + 2;
-  uint64_t* drained = qfull + 1;
-  uint64_t* looked = drained + 1;  // [2] every warp of a warpgroup has looked over a masked tile's V rows
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(looked + 2);
+  uint64_t* cfull = empty + NS;    // [NC] codes landed
+  uint64_t* cempty = cfull + NC;   // [NC] codes converted
+  uint64_t* qfull = cempty + NC;   // [2] a row tile's Q is in shared memory
+  uint64_t* qfree = qfull + 2;     // [2] its products are done
+  uint64_t* sfull = qfree + 2;     // [2] scores are in tensor memory (and the warpgroup's earlier P V is done)
+  uint64_t* pready = sfull + 2;    // [2] probabilities are
+  uint64_t* ofull = pready + 2;    // [2] the item's output is complete
+  uint64_t* looked = ofull + 2;    // [2] every warp has looked over a masked tile's V rows
+  uint64_t* mlready = looked + 2;  // the second warpgroup's (maximum, sum) are in shared memory
+  uint64_t* merged = mlready + 1;  // ... and its output has been read
+  uint64_t* drained = merged + 1;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(drained + 1);
   int* skip = reinterpret_cast<int*>(tmem_holder + 1);  // [2] the softmax threads did this tile's P V themselves
   int* odd_v = skip + 2;           // [2] an infinity or NaN was found among V rows that some row may not see
 
   griddep_launch();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  griddep_wait();
-  const RagHead* head = reinterpret_cast<const RagHead*>(p.work);
-  const int entry = (int)blockIdx.x / p.hkv, kvh = (int)blockIdx.x % p.hkv;
-  if (entry >= head->n_list) return;
-  const RagItem it = reinterpret_cast<const RagItem*>(p.work + p.list_off)[entry];
-  if (it.row0 < 0 || (int64_t)it.row0 + it.n_tok > p.rows || it.seq < 0 || it.seq >= p.b ||
-      (int64_t)it.kv_len > (int64_t)p.max_blocks * 16 || it.slot >= p.max_slots) {  // a plan for other sizes
-    if (threadIdx.x == 0) mg_record_error(MG_ERR_DEVICE, 510);
-    return;
-  }
-  // K/V tiles of each row tile: up to its last token's position (none for an empty second tile)
-  int n_w[2];
-#pragma unroll
-  for (int w = 0; w < 2; ++w) {
-    const int toks = min(p.tok_tile, it.n_tok - w * p.tok_tile);
-    const int last = it.pos0 + w * p.tok_tile + toks - 1;
-    n_w[w] = toks <= 0 ? 0 : max(0, min(it.kt1, last / kRows + 1) - it.kt0);
-  }
-  const int n_all = max(n_w[0], n_w[1]);
-
   if (threadIdx.x == 0) {
+    mg_set_error_words(p.err_code, p.err_info);
     for (int s = 0; s < NS; ++s) {
-      mbar_init(&full[s], Q8 ? 128 : 1);
+      mbar_init(&full[s], Q8 ? 4 : 1);
       mbar_init(&empty[s], 1);
     }
+    for (int s = 0; s < NC; ++s) {
+      mbar_init(&cfull[s], 1);
+      mbar_init(&cempty[s], 4);
+    }
     for (int w = 0; w < 2; ++w) {
+      mbar_init(&qfull[w], 1);
+      mbar_init(&qfree[w], 1);
       mbar_init(&sfull[w], 1);
       mbar_init(&pready[w], 4);
       mbar_init(&ofull[w], 1);
       mbar_init(&looked[w], 4);
       skip[w] = odd_v[w] = 0;
     }
-    mbar_init(qfull, 8);
+    mbar_init(mlready, 4);
+    mbar_init(merged, 4);
     mbar_init(drained, 1);
     fence_mbar_init();
   }
@@ -162,366 +314,547 @@ __global__ void __launch_bounds__(RagCfg<D, Q8>::kThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_holder;
-  const int32_t* table = p.tables + (int64_t)it.seq * p.max_blocks;
-  const int blocks = (it.kv_len + 15) >> 4;
+  const uint32_t tmem = 0;  // the CTA holds all of tensor memory
+  griddep_wait();
+  const int total = reinterpret_cast<const RagHead*>(p.work)->n_list * p.hkv;
 
   if (warp >= 8) {
-    if (warp == 9 && !Q8) {
-      // ---------------- TMA producer: K_0, V_0, K_1, V_1, ... ----------------
-      // lane = (block of the tile, slab of the row); K and V tiles of the same index use the same block ids
-      const int blk = lane & 7, slab = lane >> 3;
-      const bool mine = slab < C::kSlabs;
-      bool ok = true;
-      int i = 0;
-      for (int j = 0; j < n_all && ok; ++j) {
-        const int b0 = (it.kt0 + j) * 8, nb = min(8, blocks - b0);
-        int row = (int)(p.num_blocks * p.hkv * 16);  // behind the pool: reads zeros
-        if (blk < nb) {
-          const int32_t id = table[b0 + blk];
-          if (id >= 0 && id < p.num_blocks) row = (id * p.hkv + kvh) * 16;
-          else mg_record_error(MG_ERR_DEVICE, 511);
-        }
-        for (int kv = 0; kv < 2 && ok; ++kv, ++i) {
-          const int s = i % NS;
-          if (i >= NS) ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], ((i / NS) - 1) & 1, 512));
-          if (!ok) break;
-          if (lane == 0) mbar_arrive_expect_tx(&full[s], (uint32_t)(nb * 16 * D * 2));
-          __syncwarp();
-          if (mine && blk < nb)
-            tma_load_2d(smem + C::kRing + s * C::kTileBytes + slab * C::kSlabBytes + blk * 16 * C::kSlab,
-                        kv ? &tv : &tk, &full[s], slab * (C::kSlab / 2), row);
-        }
-      }
-      // the loads that were started have landed before this CTA's memory goes to another
-      for (int k = max(0, i - NS); k < i; ++k) mbar_wait(&full[k % NS], (k / NS) & 1, 513);
-    } else if (warp == 8) {
+    regs_dec<C::kOtherRegs>();
+    bool ok = true;
+    int index = rag_index(0, total);
+    RagItem next = rag_item(p, index);
+    if (warp == 8) {
       // ---------------- tensor-core issue ----------------
-      if (lane == 0) {
-        bool ok = mbar_wait(qfull, 0, 514);
-        const uint32_t sq = smem_u32(smem + C::kQ), sr = smem_u32(smem + C::kRing);
-        auto scores = [&](int w, int j) {  // S_w = Q_w K_j^T
-          const uint32_t a = sq + (uint32_t)(w * C::kTileBytes), k = sr + (uint32_t)((2 * j % NS) * C::kTileBytes);
+      const uint32_t sq = smem_u32(smem), sr = smem_u32(smem + C::kRing);
+      const uint64_t q_desc = rag_desc<D>(sq, 16), k_desc = rag_desc<D>(sr, 16), v_desc = rag_desc<D>(sr, C::kSlabBytes);
+      int base = 0;
+      uint32_t pp = 0, pq = 0;  // phase bits of pready and qfull, one per row tile
+      for (int k = 0; index >= 0 && ok; ++k) {
+        const RagWork wk = rag_work(p, next, index);
+        index = rag_index(k + 1, total);
+        next = rag_item(p, index);
+        const int tiles = uniform(wk.tiles), n0 = uniform(wk.n0), n1 = uniform(wk.n1);
+        const bool dual = uniform(wk.dual) != 0;
+        // S_w = Q_w K_j^T (in a branch of one thread)
+        auto scores = [&](int w, int j) {
+          const uint64_t a = q_desc + (uint64_t)(w * (C::kTileBytes >> 4));
+          const uint64_t b = k_desc + (uint64_t)(((base + 2 * j) % NS) * (C::kTileBytes >> 4));
 #pragma unroll
           for (int x = 0; x < D / 16; ++x) {
-            const uint32_t off = (uint32_t)((x * 32 / C::kSlab) * C::kSlabBytes + (x * 32) % C::kSlab);
-            tc_mma_ss(tmem + (uint32_t)(w * kRows), rag_desc<D>(a + off, 16), rag_desc<D>(k + off, 16), C::kIdescS,
-                      x > 0);
+            const uint64_t off = (uint64_t)(((x * 32 / C::kSlab) * C::kSlabBytes + (x * 32) % C::kSlab) >> 4);
+            tc_mma_ss((uint32_t)(w * kRows), a + off, b + off, C::kIdescS, x > 0);
           }
           tc_commit(&sfull[w]);
         };
-        if (ok && n_all > 0) {
-          ok = mbar_wait(&full[0], 0, 515);
+        auto await_k = [&](int j) {
+          const int i = base + 2 * j;
+          ok = ok && bar_wait(&full[i % NS], (i / NS) & 1, 515);
           tc_fence_after();
-          if (ok) {
-            if (n_w[0] > 0) scores(0, 0);
-            if (n_w[1] > 0) scores(1, 0);
-            tc_commit(&empty[0]);
-          }
-        }
-        for (int j = 0; j < n_all && ok; ++j) {
-          const int sv = (2 * j + 1) % NS, sk = (2 * j + 2) % NS;
-          for (int w = 0; w < 2 && ok; ++w) {
-            if (j >= n_w[w]) continue;
-            ok = mbar_wait(&full[sv], ((2 * j + 1) / NS) & 1, 516) && mbar_wait(&pready[w], j & 1, 517);
-            if (!ok) break;
-            tc_fence_after();
-            if (!*(volatile int*)&skip[w]) {
-              const uint32_t v = sr + (uint32_t)(sv * C::kTileBytes);
+        };
+        const int step = dual ? 2 : 1;
 #pragma unroll
-              for (int x = 0; x < kRows / 16; ++x)  // 16 keys a step: 16 rows of V
-                tc_mma_ts(tmem + C::kO + (uint32_t)(w * D), tmem + (uint32_t)(w * kRows + x * 8),
-                          rag_desc<D>(v + (uint32_t)(x * 16 * C::kSlab), C::kSlabBytes), C::kIdescO, j > 0 || x > 0);
+        for (int w = 0; w < 2; ++w) {
+          const int n = w ? n1 : n0;
+          if (n == 0 || !ok) continue;
+          ok = bar_wait(&qfull[w], (pq >> w) & 1, 514);
+          pq ^= 1u << w;
+          const int j = dual ? w : 0;
+          if (dual || w == 0 || n0 == 0) await_k(j);
+          if (!ok) break;
+          if (elect_one()) {
+            scores(w, j);
+            if (n == 1) tc_commit(&qfree[w]);
+            if (dual || w == 1) tc_commit(&empty[(base + 2 * j) % NS]);
+          }
+          __syncwarp();
+        }
+        for (int j = 0; j < tiles && ok; ++j) {
+          const int iv = base + 2 * j + 1, jn = j + step;
+          const uint64_t v = v_desc + (uint64_t)((iv % NS) * (C::kTileBytes >> 4));
+          ok = bar_wait(&full[iv % NS], (iv / NS) & 1, 516);
+          bool k_here = false;
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            const int last = dual ? tiles : (w ? n1 : n0);
+            if (!ok || (dual ? w != (j & 1) : j >= last)) continue;
+            ok = bar_wait(&pready[w], (pp >> w) & 1, 517);
+            if (!ok) break;
+            pp ^= 1u << w;
+            tc_fence_after();
+            const bool by_hand = !Q8 && uniform(*(volatile int*)&skip[w]) != 0;
+            if (elect_one()) {
+              if (!by_hand) {
+                const uint32_t more = j >= step;  // something is in O already
+#pragma unroll
+                for (int x = 0; x < kRows / 16; ++x)  // 16 keys a step: 16 rows of V
+                  tc_mma_ts(C::kO + (uint32_t)(w * D), (uint32_t)(w * kRows + x * 8),
+                            v + (uint64_t)((x * 16 * C::kSlab) >> 4), C::kIdescO, x > 0 ? 1u : more);
+              }
+              if (dual || w == 1) tc_commit(&empty[iv % NS]);
+              if (jn >= last) tc_commit(&ofull[w]);
             }
-            if (j + 1 < n_w[w]) {
-              ok = mbar_wait(&full[sk], ((2 * j + 2) / NS) & 1, 518);
+            __syncwarp();
+            if (jn < last) {
+              if (!k_here) await_k(jn);
+              k_here = true;
               if (!ok) break;
-              tc_fence_after();
-              scores(w, j + 1);
-            } else {
-              tc_commit(&ofull[w]);
+              if (elect_one()) {
+                scores(w, jn);
+                if (jn + step >= last) tc_commit(&qfree[w]);
+                if (dual || w == 1) tc_commit(&empty[(base + 2 * jn) % NS]);
+              }
+              __syncwarp();
             }
           }
-          if (!ok) break;
-          tc_commit(&empty[sv]);
-          if (j + 1 < n_all) tc_commit(&empty[sk]);
         }
-        tc_commit(drained);
-        mbar_wait(drained, 0, 519);
+        base += 2 * tiles;
       }
-    } else if (Q8 && warp >= 9) {
-      // ---------------- int8 codes -> bf16 tiles ----------------
-      const int t = threadIdx.x - 9 * 32;
+      if (elect_one()) tc_commit(drained);
+      __syncwarp();
+      bar_wait(drained, 0, 519);
+    } else if (warp == 9) {
+      // ---------------- K/V loads: K_0, V_0, K_1, V_1, ... ----------------
+      // bf16: a TMA copy for each block and slab; int8: bulk copies of a block's codes and scales. Lane b < 8 holds the
+      // tile's b-th block id, fetched a tile ahead; one lane starts the copies
+      int i = 0;
+      const int blk = lane & 7;
+      for (int k = 0; index >= 0 && ok; ++k) {
+        const RagWork wk = rag_work(p, next, index);
+        if (wk.it.n_tok == 0) mg_record_error(MG_ERR_DEVICE, 510);
+        index = rag_index(k + 1, total);
+        next = rag_item(p, index);
+        const int32_t* table = p.tables + (int64_t)wk.it.seq * p.max_blocks;
+        const int blocks = (wk.it.kv_len + 15) >> 4;
+        int b0 = wk.it.kt0 * 8;
+        int32_t id_next = wk.tiles > 0 && b0 + blk < blocks ? table[b0 + blk] : 0;
+        for (int j = 0; j < wk.tiles && ok; ++j, b0 += 8) {
+          const int nb = min(8, blocks - b0);
+          const int32_t id = id_next;
+          const bool good = id >= 0 && id < p.num_blocks;
+          if (blk < nb && !good) mg_record_error(MG_ERR_DEVICE, 511);
+          if (b0 + 8 + blk < blocks) id_next = table[b0 + 8 + blk];
+#pragma unroll
+          for (int kv = 0; kv < 2; ++kv, ++i) {
+            if constexpr (Q8) {
+              const int s = i % NC;
+              if (i >= NC) ok = ok && bar_wait(&cempty[s], ((i / NC) - 1) & 1, 512);
+              if (!ok) break;
+              // a block that is not in the pool is read as the pool's first (its error has been recorded)
+              const int row = (good ? id : 0) * p.hkv + wk.head;
+              if (elect_one()) mbar_arrive_expect_tx(&cfull[s], (uint32_t)(nb * 16 * (D + 4)));
+#pragma unroll
+              for (int y = 0; y < 8; ++y) {
+                const int64_t r = (int64_t)__shfl_sync(0xffffffffu, row, y) * 16;
+                if (y < nb && elect_one()) {
+                  bulk_load_smem(smem + C::kCodes + s * C::kCodeBytes + y * 16 * D, (kv ? p.v8 : p.k8) + r * D, 16 * D,
+                                 &cfull[s]);
+                  bulk_load_smem(smem + C::kCodeScales + s * kRows * 4 + y * 64, (kv ? p.vs : p.ks) + r, 64, &cfull[s]);
+                }
+                __syncwarp();
+              }
+            } else {
+              const int s = i % NS;
+              if (i >= NS) ok = ok && bar_wait(&empty[s], ((i / NS) - 1) & 1, 512);
+              if (!ok) break;
+              // (a block that is not in the pool is read behind its end: as zeros)
+              const int row = (int)(good ? (id * p.hkv + wk.head) * 16 : p.num_blocks * p.hkv * 16);
+              if (elect_one()) mbar_arrive_expect_tx(&full[s], (uint32_t)(nb * 16 * D * 2));
+#pragma unroll
+              for (int y = 0; y < 8; ++y) {
+                const int r = __shfl_sync(0xffffffffu, row, y);
+                if (y < nb && elect_one()) {
+#pragma unroll
+                  for (int x = 0; x < C::kSlabs; ++x)
+                    tma_load_2d(smem + C::kRing + s * C::kTileBytes + x * C::kSlabBytes + y * 16 * C::kSlab, kv ? &tv : &tk,
+                                &full[s], x * (C::kSlab / 2), r);
+                }
+                __syncwarp();
+              }
+            }
+          }
+        }
+      }
+      // the loads that were started have landed before this CTA's memory goes to another
+      if constexpr (Q8) {
+        for (int x = max(0, i - NC); x < i; ++x) bar_wait(&cfull[x % NC], (x / NC) & 1, 513);
+      } else {
+        for (int x = max(0, i - NS); x < i; ++x) bar_wait(&full[x % NS], (x / NS) & 1, 513);
+      }
+    } else if (warp == 10) {
+      // ---------------- Q loads: a row tile's tokens x heads of the group, as soon as the products before are done ------
+      int c0 = 0, c1 = 0;  // loads so far
+      for (int k = 0; index >= 0 && ok; ++k) {
+        const RagWork wk = rag_work(p, next, index);
+        index = rag_index(k + 1, total);
+        next = rag_item(p, index);
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          int& c = w ? c1 : c0;
+          if ((w ? wk.n1 : wk.n0) == 0 || !ok) continue;
+          if (c > 0) ok = bar_wait(&qfree[w], (c - 1) & 1, 524);
+          if (!ok) break;
+          ++c;
+          if (elect_one()) {
+            mbar_arrive_expect_tx(&qfull[w], (uint32_t)(C::kSlabs * p.tok_tile * p.group * C::kSlab));
+#pragma unroll
+            for (int s = 0; s < C::kSlabs; ++s)
+              tma_load_3d(smem + w * C::kTileBytes + s * C::kSlabBytes, &tq, &qfull[w], s * (C::kSlab / 2),
+                          wk.head * p.group, wk.it.row0 + (wk.dual ? 0 : w * p.tok_tile));
+          }
+          __syncwarp();
+        }
+      }
+      if (c0 > 0) bar_wait(&qfull[0], (c0 - 1) & 1, 525);
+      if (c1 > 0) bar_wait(&qfull[1], (c1 - 1) & 1, 525);
+    } else if (Q8 && warp >= 12) {
+      // ---------------- int8 codes -> bf16 tiles, swizzled ----------------
+      const int t = threadIdx.x - 12 * 32;
       float* scales = reinterpret_cast<float*>(smem + C::kScales);
       constexpr int kParts = D / 16;              // 16-byte pieces of a vector of codes
       constexpr int kPer = kRows * kParts / 128;  // pieces per thread and tile
-      bool ok = true;
-      int i = 0;
-      for (int j = 0; j < n_all && ok; ++j) {
-        const int key0 = (it.kt0 + j) * kRows;
-        for (int kv = 0; kv < 2 && ok; ++kv, ++i) {
-          const int s = i % NS;
-          const int8_t* pool = kv ? p.v8 : p.k8;
-          uint4 c[kPer];
+      int i = 0, tile = 0;
+      for (int k = 0; index >= 0 && ok; ++k) {
+        const RagWork wk = rag_work(p, next, index);
+        index = rag_index(k + 1, total);
+        next = rag_item(p, index);
+        for (int j = 0; j < wk.tiles && ok; ++j, ++tile) {
+          const int keys = wk.it.kv_len - (wk.it.kt0 + j) * kRows;  // of the tile, where fewer than 128
+#pragma unroll 1
+          for (int kv = 0; kv < 2; ++kv, ++i) {
+            const int s = i % NS, sc = i % NC;
+            ok = ok && bar_wait(&cfull[sc], (i / NC) & 1, 526);
+            if (i >= NS) ok = ok && bar_wait(&empty[s], ((i / NS) - 1) & 1, 527);
+            if (!ok) break;
+            const uint8_t* src = smem + C::kCodes + sc * C::kCodeBytes;
+            uint8_t* dst = smem + C::kRing + s * C::kTileBytes;
 #pragma unroll
-          for (int x = 0; x < kPer; ++x) {  // all loads first
-            const int piece = x * 128 + t, key = key0 + piece / kParts;
-            c[x] = make_uint4(0, 0, 0, 0);
-            if (key < it.kv_len) {
-              const int32_t id = table[key >> 4];
-              if (id >= 0 && id < p.num_blocks)
-                c[x] = *reinterpret_cast<const uint4*>(
-                    pool + (((int64_t)id * p.hkv + kvh) * 16 + (key & 15)) * D + (piece % kParts) * 16);
-              else mg_record_error(MG_ERR_DEVICE, 511);
+            for (int x = 0; x < kPer; ++x) {
+              const int piece = x * 128 + t, r = piece / kParts, q = (piece % kParts) * 2;
+              uint4 c = make_uint4(0, 0, 0, 0);
+              if (r < keys) c = *reinterpret_cast<const uint4*>(src + piece * 16);
+              uint4 lo, hi;
+              i8x4_to_bf16x4(c.x, lo.x, lo.y);
+              i8x4_to_bf16x4(c.y, lo.z, lo.w);
+              i8x4_to_bf16x4(c.z, hi.x, hi.y);
+              i8x4_to_bf16x4(c.w, hi.z, hi.w);
+              *reinterpret_cast<uint4*>(dst + chunk_at<D>(r, q)) = lo;
+              *reinterpret_cast<uint4*>(dst + chunk_at<D>(r, q + 1)) = hi;
+            }
+            scales[(tile % C::kScaleRing) * 2 * kRows + kv * kRows + t] =
+                t < keys ? reinterpret_cast<const float*>(smem + C::kCodeScales)[sc * kRows + t] : 0.f;
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              mbar_arrive(&cempty[sc]);
+              mbar_arrive(&full[s]);
             }
           }
-          float sc = 0.f;
-          if (key0 + t < it.kv_len) {
-            const int32_t id = table[(key0 + t) >> 4];
-            if (id >= 0 && id < p.num_blocks)
-              sc = (kv ? p.vs : p.ks)[((int64_t)id * p.hkv + kvh) * 16 + ((key0 + t) & 15)];
-          }
-          if (i >= NS) ok = mbar_wait(&empty[s], ((i / NS) - 1) & 1, 512);
-          if (!ok) break;
-          uint8_t* dst = smem + C::kRing + s * C::kTileBytes;
-#pragma unroll
-          for (int x = 0; x < kPer; ++x) {
-            const int piece = x * 128 + t, r = piece / kParts, q = (piece % kParts) * 2;
-            uint4 lo, hi;
-            i8x4_to_bf16x4(c[x].x, lo.x, lo.y);
-            i8x4_to_bf16x4(c[x].y, lo.z, lo.w);
-            i8x4_to_bf16x4(c[x].z, hi.x, hi.y);
-            i8x4_to_bf16x4(c[x].w, hi.z, hi.w);
-            *reinterpret_cast<uint4*>(dst + chunk_at<D>(r, q)) = lo;
-            *reinterpret_cast<uint4*>(dst + chunk_at<D>(r, q + 1)) = hi;
-          }
-          scales[(j % C::kScaleRing) * 2 * kRows + kv * kRows + t] = sc;
-          fence_async_smem();
-          mbar_arrive(&full[s]);
         }
       }
     }
   } else {
     // ---------------- softmax: one thread per row ----------------
-    const int w = warp >> 2, t = threadIdx.x & 127;  // row tile, row
-    const int valid = max(0, min(p.tok_tile, it.n_tok - w * p.tok_tile)) * p.group;
-    const int tok0 = w * p.tok_tile;
+    regs_inc<C::kSoftRegs>();
+    const int w = warp >> 2, t = threadIdx.x & 127;  // warpgroup, row
+    const int my_tok = t / p.group;
     const int64_t row_stride = (int64_t)p.hq * D;
-    const int64_t base = (int64_t)(it.row0 + tok0) * row_stride + (int64_t)kvh * p.group * D;
-    {  // this tile's rows of Q into shared memory (rows that are not there as zeros)
-      constexpr int kChunks = D / 8;
-#pragma unroll 8
-      for (int x = 0; x < kRows * kChunks / 128; ++x) {
-        const int idx = x * 128 + t, r = idx / kChunks, c = idx % kChunks;
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (r < valid)
-          v = *reinterpret_cast<const uint4*>(p.q + base + (int64_t)(r / p.group) * row_stride + (r % p.group) * D + c * 8);
-        *reinterpret_cast<uint4*>(smem + C::kQ + w * C::kTileBytes + chunk_at<D>(r, c)) = v;
-      }
-      fence_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(qfull);
-    }
+    const int64_t my_off = (int64_t)my_tok * row_stride + (t % p.group) * D;
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t ts = tmem + lane_base + (uint32_t)(w * kRows), to = tmem + lane_base + C::kO + (uint32_t)(w * D);
-    const int first_pos = it.pos0 + tok0, my_pos = first_pos + t / p.group;
-    const bool warp_on = (warp & 3) * 32 < valid;
-    float m = -INFINITY, l = 0.f;  // m: the maximum in use, in score units
+    const uint64_t scale2 = pair(p.scale_log2, p.scale_log2);
     bool ok = true;
-    int looks = 0;
-    for (int j = 0; j < n_w[w] && ok; ++j) {
-      const int key0 = (it.kt0 + j) * kRows;
-      ok = __all_sync(0xffffffffu, mbar_wait(&sfull[w], j & 1, 520));
-      if (!ok) break;
-      tc_fence_after();
-      const bool masked = key0 + kRows - 1 > first_pos;  // some row of the tile does not see all its keys
-      bool by_hand = false;
-      if constexpr (!Q8) {
-        if (masked) {
-          // V rows that some row may not see: zero those behind the item's keys, look the others over
-          const int sv = (2 * j + 1) % NS;
-          ok = __all_sync(0xffffffffu, mbar_wait(&full[sv], ((2 * j + 1) / NS) & 1, 521));
+    int base = 0, cs = 0, co = 0, looks = 0, duals = 0, tile0 = 0;
+    int index = rag_index(0, total);
+    RagItem next = rag_item(p, index);
+    for (int k = 0; index >= 0 && ok; ++k) {
+      const RagWork wk = rag_work(p, next, index);
+      index = rag_index(k + 1, total);
+      next = rag_item(p, index);
+      const RagItem& it = wk.it;
+      const int tok0 = wk.dual ? 0 : w * p.tok_tile;
+      const int valid = max(0, min(p.tok_tile, it.n_tok - tok0)) * p.group;
+      const int first_pos = it.pos0 + tok0, my_pos = first_pos + my_tok;
+      const bool warp_on = (warp & 3) * 32 < valid;
+      const int n = w ? wk.n1 : wk.n0;
+      float m = -INFINITY;  // the maximum in use, in score units
+      uint64_t l2 = 0;      // the sum, in two halves
+      for (int i = 0; i < n && ok; ++i) {
+        const int j = wk.dual ? 2 * i + w : i;
+        const int key0 = (it.kt0 + j) * kRows;
+        ok = bar_wait(&sfull[w], cs++ & 1, 520);
+        if (!ok) break;
+        tc_fence_after();
+        const bool masked = key0 + kRows - 1 > first_pos;  // some row of the tile does not see all its keys
+        bool by_hand = false;
+        if constexpr (Q8) {  // the values' scales come with V
+          const int iv = base + 2 * j + 1;
+          ok = bar_wait(&full[iv % NS], (iv / NS) & 1, 521);
           if (!ok) break;
-          uint8_t* v = smem + C::kRing + sv * C::kTileBytes;
-          const int r_first = max(0, first_pos + 1 - key0), r_end = min(kRows, it.kv_len - key0);
-          bool odd = false;
-          for (int x = r_first * (D / 8) + t; x < kRows * (D / 8); x += 128) {
-            const int r = x / (D / 8);
-            uint4* at = reinterpret_cast<uint4*>(v + chunk_at<D>(r, x % (D / 8)));
-            if (r >= r_end) {
-              *at = make_uint4(0, 0, 0, 0);
-            } else {
-              const uint4 q = *at;
-              const uint32_t e[4] = {q.x, q.y, q.z, q.w};
+        } else {
+          if (i == 0 && t == 0) *(volatile int*)&odd_v[w] = 0;
+          if (masked) {
+            // V rows that some row may not see: zero those behind the item's keys, look the others over
+            const int iv = base + 2 * j + 1, sv = iv % NS;
+            ok = bar_wait(&full[sv], (iv / NS) & 1, 521);
+            if (!ok) break;
+            uint8_t* v = smem + C::kRing + sv * C::kTileBytes;
+            const int r_first = max(0, first_pos + 1 - key0), r_end = min(kRows, it.kv_len - key0);
+            // (a bf16 infinity or NaN has all exponent bits set: adding one at the lowest of them carries out)
+            uint32_t acc = 0;
+            constexpr int kChunks = D / 8, kBatch = 4;
+            for (int x0 = r_first * kChunks + t; x0 < kRows * kChunks; x0 += 128 * kBatch) {
+              uint4 q[kBatch];
 #pragma unroll
-              for (int y = 0; y < 4; ++y)
-                odd |= (e[y] & 0x7f800000u) == 0x7f800000u || (e[y] & 0x7f80u) == 0x7f80u;
+              for (int y = 0; y < kBatch; ++y) {
+                const int x = x0 + y * 128;
+                q[y] = make_uint4(0, 0, 0, 0);
+                if (x < r_end * kChunks) q[y] = *reinterpret_cast<const uint4*>(v + chunk_at<D>(x / kChunks, x % kChunks));
+              }
+#pragma unroll
+              for (int y = 0; y < kBatch; ++y) {
+                const int x = x0 + y * 128;
+                if (x >= r_end * kChunks && x < kRows * kChunks)
+                  *reinterpret_cast<uint4*>(v + chunk_at<D>(x / kChunks, x % kChunks)) = make_uint4(0, 0, 0, 0);
+                acc |= ((q[y].x & 0x7f807f80u) + 0x00800080u) | ((q[y].y & 0x7f807f80u) + 0x00800080u) |
+                       ((q[y].z & 0x7f807f80u) + 0x00800080u) | ((q[y].w & 0x7f807f80u) + 0x00800080u);
+              }
+            }
+            bool odd = (acc & 0x80008000u) != 0;
+            fence_async_smem();
+            // (any thread's finding is every thread's; once found it holds for the item's later tiles too)
+            odd = __any_sync(0xffffffffu, odd);
+            if (lane == 0) {
+              if (odd) *(volatile int*)&odd_v[w] = 1;
+              mbar_arrive(&looked[w]);
+            }
+            ok = bar_wait(&looked[w], looks & 1, 523);
+            ++looks;
+            if (!ok) break;
+            by_hand = *(volatile int*)&odd_v[w] != 0;
+          }
+        }
+        if (warp_on) {
+          float s[kRows];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tmem_ld32(ts + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&s[c * 32]));
+          tc_wait_ld();
+          const float* sc = reinterpret_cast<const float*>(smem + C::kScales) + ((tile0 + j) % C::kScaleRing) * 2 * kRows;
+          if constexpr (Q8) {
+#pragma unroll
+            for (int c = 0; c < kRows; c += 4) {
+              const float4 f = *reinterpret_cast<const float4*>(sc + c);
+              s[c] *= f.x, s[c + 1] *= f.y, s[c + 2] *= f.z, s[c + 3] *= f.w;
             }
           }
-          fence_async_smem();
-          // (any thread's finding is every thread's; once found it holds for the item's later tiles too)
-          odd = __any_sync(0xffffffffu, odd);
-          if (lane == 0) {
-            if (odd) *(volatile int*)&odd_v[w] = 1;
-            mbar_arrive(&looked[w]);
+          const int see = my_pos - key0;  // keys 0 .. see of the tile are this row's
+          if (masked) {
+#pragma unroll
+            for (int c = 0; c < kRows; ++c) s[c] = c <= see ? s[c] : -INFINITY;
           }
-          ok = __all_sync(0xffffffffu, mbar_wait(&looked[w], looks & 1, 523));
-          ++looks;
-          if (!ok) break;
-          by_hand = *(volatile int*)&odd_v[w] != 0;
-        }
-      }
-      if (warp_on) {
-        float s[kRows];
+          float mx[8];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld32(ts + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&s[c * 32]));
-        tc_wait_ld();
-        const float* sc = reinterpret_cast<const float*>(smem + C::kScales) + (j % C::kScaleRing) * 2 * kRows;
-        if constexpr (Q8) {
+          for (int c = 0; c < 8; ++c) mx[c] = fmaxf(s[c], s[c + 8]);
 #pragma unroll
-          for (int c = 0; c < kRows; c += 4) {
-            const float4 f = *reinterpret_cast<const float4*>(sc + c);
-            s[c] *= f.x, s[c + 1] *= f.y, s[c + 2] *= f.z, s[c + 3] *= f.w;
+          for (int c = 16; c < kRows; c += 16) {
+#pragma unroll
+            for (int x = 0; x < 8; ++x) mx[x] = fmaxf(fmaxf(mx[x], s[c + x]), s[c + 8 + x]);
           }
-        }
-        const int see = my_pos - key0;  // keys 0 .. see of the tile are this row's
-        if (masked) {
-#pragma unroll
-          for (int c = 0; c < kRows; ++c) s[c] = c <= see ? s[c] : -INFINITY;
-        }
-        float mx = s[0];
-#pragma unroll
-        for (int c = 1; c < kRows; ++c) mx = fmaxf(mx, s[c]);
-        float m_new = fmaxf(m, mx);
-        const bool grow = m == -INFINITY || (m_new - m) * p.scale_log2 > 8.f;
-        if (!grow) m_new = m;
-        if (__any_sync(0xffffffffu, grow) && j > 0) {
-          const float f = m == -INFINITY ? 0.f : ex2((m - m_new) * p.scale_log2);
-          l *= f;
-#pragma unroll
-          for (int c = 0; c < D; c += 32) {
-            uint32_t o[32];
-            tmem_ld32(to + c, o);
-            tc_wait_ld();
-#pragma unroll
-            for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
-            tmem_st32(to + c, o);
-          }
-          tc_wait_st();
-        }
-        m = m_new;
-        const float off = m == -INFINITY ? 0.f : m * p.scale_log2;
-        float sum = 0.f;
-        uint32_t pk[32];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-#pragma unroll
-          for (int c = 0; c < 64; c += 2) {
-            float a = ex2(fmaf(s[h * 64 + c], p.scale_log2, -off)), b = ex2(fmaf(s[h * 64 + c + 1], p.scale_log2, -off));
-            sum += a + b;
-            if constexpr (Q8) {  // the value's scale, with nothing of a masked key's
-              a = !masked || h * 64 + c <= see ? a * sc[kRows + h * 64 + c] : 0.f;
-              b = !masked || h * 64 + c + 1 <= see ? b * sc[kRows + h * 64 + c + 1] : 0.f;
-            }
-            pk[c / 2] = pack_bf16x2(a, b);
-          }
-          tmem_st32(ts + h * 32, pk);
-        }
-        l += sum;
-        tc_wait_st();
-        if constexpr (!Q8) {
-          if (by_hand) {
-            // O += P V over the keys that each row sees, from the stage, in the tensor cores' place
-            const uint8_t* v = smem + C::kRing + ((2 * j + 1) % NS) * C::kTileBytes;
+          float m_new = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7])));
+          m_new = fmaxf(m, m_new);
+          const bool grow = m == -INFINITY || (m_new - m) * p.scale_log2 > 8.f;
+          if (!grow) m_new = m;
+          if (i > 0 && __any_sync(0xffffffffu, grow)) {
+            const float f = m == -INFINITY ? 0.f : ex2((m - m_new) * p.scale_log2);
+            l2 = mul2(l2, pair(f, f));
 #pragma unroll 1
             for (int c = 0; c < D; c += 32) {
               uint32_t o[32];
-              if (j > 0) {
-                tmem_ld32(to + c, o);
-                tc_wait_ld();
+              tmem_ld32(to + c, o);
+              tc_wait_ld();
+#pragma unroll
+              for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
+              tmem_st32(to + c, o);
+            }
+          }
+          m = m_new;
+          const float off = m == -INFINITY ? 0.f : -m * p.scale_log2;
+          const uint64_t off2 = pair(off, off);
+          uint64_t sum[2] = {l2, 0};
+#pragma unroll
+          for (int h = 0; h < 4; ++h) {
+            uint32_t pk[16];
+#pragma unroll
+            for (int c = 0; c < 16; ++c) {
+              const int e = h * 32 + 2 * c;
+              const uint64_t x = fma2(pair(s[e], s[e + 1]), scale2, off2);
+              uint64_t y;
+              float a, b;
+              if (C::kPolyEvery > 0 && (c % (C::kPolyEvery > 0 ? C::kPolyEvery : 1)) == 1) {
+                y = ex2_poly2(x);
+                unpair(y, a, b);
+                if (masked) {  // exactly zero
+                  a = e <= see ? a : 0.f;
+                  b = e + 1 <= see ? b : 0.f;
+                  y = pair(a, b);
+                }
               } else {
-#pragma unroll
-                for (int x = 0; x < 32; ++x) o[x] = 0;
+                unpair(x, a, b);
+                a = ex2(a);
+                b = ex2(b);
+                y = pair(a, b);
               }
+              sum[c & 1] = add2(sum[c & 1], y);
+              if constexpr (Q8) {  // the value's scale, with nothing of a masked key's
+                unpair(mul2(y, *reinterpret_cast<const uint64_t*>(sc + kRows + e)), a, b);
+                if (masked) {
+                  a = e <= see ? a : 0.f;
+                  b = e + 1 <= see ? b : 0.f;
+                }
+              }
+              pk[c] = pack_bf16x2(a, b);
+            }
+            tmem_st16(ts + h * 16, pk);
+          }
+          l2 = add2(sum[0], sum[1]);
+          tc_wait_st();
+          if constexpr (!Q8) {
+            if (by_hand) {
+              // O += P V over the keys that each row sees, from the stage, in the tensor cores' place
+              const uint8_t* v = smem + C::kRing + ((base + 2 * j + 1) % NS) * C::kTileBytes;
 #pragma unroll 1
-              for (int k = 0; k < kRows; k += 64) {
-                uint32_t pr[32];
-                tmem_ld32(ts + k / 2, pr);
-                tc_wait_ld();
+              for (int c = 0; c < D; c += 8) {
+                float o[8];
+                uint32_t u[8];
+                if (i > 0) {
+                  tmem_ld8(to + c, u);
+                  tc_wait_ld();
+                } else {
 #pragma unroll
-                for (int kk = 0; kk < 64; ++kk) {
-                  const float pv = kk & 1 ? bf16hi(pr[kk / 2]) : bf16lo(pr[kk / 2]);
-                  if (k + kk <= see) {
+                  for (int x = 0; x < 8; ++x) u[x] = 0;
+                }
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) {
-                      const uint4 q = *reinterpret_cast<const uint4*>(v + chunk_at<D>(k + kk, c / 8 + x));
-                      const uint32_t e[4] = {q.x, q.y, q.z, q.w};
+                for (int x = 0; x < 8; ++x) o[x] = __uint_as_float(u[x]);
+#pragma unroll 1
+                for (int q = 0; q < kRows; q += 16) {
+                  uint32_t pr[8];
+                  tmem_ld8(ts + q / 2, pr);
+                  tc_wait_ld();
 #pragma unroll
-                      for (int y = 0; y < 4; ++y) {
-                        o[x * 8 + 2 * y] = __float_as_uint(fmaf(pv, bf16lo(e[y]), __uint_as_float(o[x * 8 + 2 * y])));
-                        o[x * 8 + 2 * y + 1] =
-                            __float_as_uint(fmaf(pv, bf16hi(e[y]), __uint_as_float(o[x * 8 + 2 * y + 1])));
+                  for (int y = 0; y < 16; ++y) {
+                    const float pv = y & 1 ? bf16hi(pr[y / 2]) : bf16lo(pr[y / 2]);
+                    if (q + y <= see) {
+                      const uint4 x4 = *reinterpret_cast<const uint4*>(v + chunk_at<D>(q + y, c / 8));
+                      const uint32_t e[4] = {x4.x, x4.y, x4.z, x4.w};
+#pragma unroll
+                      for (int x = 0; x < 4; ++x) {
+                        o[2 * x] = fmaf(pv, bf16lo(e[x]), o[2 * x]);
+                        o[2 * x + 1] = fmaf(pv, bf16hi(e[x]), o[2 * x + 1]);
                       }
                     }
                   }
                 }
+#pragma unroll
+                for (int x = 0; x < 8; ++x) u[x] = __float_as_uint(o[x]);
+                tmem_st8(to + c, u);
               }
-              tmem_st32(to + c, o);
+              tc_wait_st();
             }
-            tc_wait_st();
           }
         }
+        if (!Q8 && t == 0) *(volatile int*)&skip[w] = by_hand;
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&pready[w]);
       }
-      if (t == 0) *(volatile int*)&skip[w] = by_hand;
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&pready[w]);
-    }
-    // ---------------- epilogue ----------------
-    if (n_w[w] > 0 && ok) ok = __all_sync(0xffffffffu, mbar_wait(&ofull[w], 0, 522));
-    if (warp_on) {
+      base += 2 * wk.tiles;
+      tile0 += wk.tiles;
+      if (!ok) break;
+      // ---------------- epilogue ----------------
+      float la, lb;
+      unpair(l2, la, lb);
+      float l = la + lb, ml = m == -INFINITY ? -INFINITY : m * p.scale_log2;
+      const bool both = wk.dual && wk.n1 > 0;  // two states of the same rows: the first warpgroup merges them
+      float2* mls = reinterpret_cast<float2*>(smem + C::kMl);
+      if (both && w == 1) {
+        mls[t] = make_float2(ml, l);
+        ok = bar_wait(&ofull[1], co++ & 1, 522);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(mlready);
+        ok = ok && bar_wait(merged, duals++ & 1, 528);
+        if (!ok) break;
+        tc_fence_after();
+        continue;
+      }
+      if (n == 0) {  // a part of a split item whose keys lie behind all of the first row tile's: an empty state
+        if (it.slot >= 0 && t < valid)
+          p.ws_ml[((int64_t)it.slot * p.hkv + wk.head) * (2 * kRows) + w * kRows + t] = make_float2(-INFINITY, 0.f);
+        continue;
+      }
+      ok = bar_wait(&ofull[w], co++ & 1, 522);
+      float f0 = 1.f, f1 = 0.f;
+      if (both) {
+        ok = ok && bar_wait(mlready, duals++ & 1, 529);
+        const float2 o1 = mls[t];
+        const float top = fmaxf(ml, o1.x);
+        f0 = ml == -INFINITY ? 0.f : exp2f(ml - top);
+        f1 = o1.x == -INFINITY ? 0.f : exp2f(o1.x - top);
+        l = (f0 == 0.f ? 0.f : f0 * l) + (f1 == 0.f ? 0.f : f1 * o1.y);
+        ml = top;
+      }
+      if (!ok) break;
       tc_fence_after();
-      const bool any = n_w[w] > 0 && ok;
-      const float inv = l == 0.f ? 0.f : 1.f / l;
-      const int64_t slot_row = ((int64_t)it.slot * p.hkv + kvh) * (2 * kRows) + w * kRows + t;
-      __nv_bfloat16* dst = p.out + base + (int64_t)(t / p.group) * row_stride + (t % p.group) * D;
+      if (warp_on) {
+        const float inv = it.slot >= 0 ? 1.f : (l == 0.f ? 0.f : 1.f / l);
+        f0 *= inv;
+        f1 *= inv;
+        const int64_t slot_row = ((int64_t)it.slot * p.hkv + wk.head) * (2 * kRows) + (wk.dual ? 0 : w * kRows) + t;
+        __nv_bfloat16* dst = p.out + (int64_t)(it.row0 + tok0) * row_stride + (int64_t)wk.head * p.group * D + my_off;
 #pragma unroll 1
-      for (int c = 0; c < D; c += 32) {
-        uint32_t o[32];
-        if (any) {
+        for (int c = 0; c < D; c += 32) {
+          uint32_t o[32];
           tmem_ld32(to + c, o);
           tc_wait_ld();
-        } else {
 #pragma unroll
-          for (int x = 0; x < 32; ++x) o[x] = 0;
-        }
-        if (t < valid) {
-          if (it.slot < 0) {
+          for (int x = 0; x < 32; ++x) o[x] = f0 == 0.f ? 0u : __float_as_uint(__uint_as_float(o[x]) * f0);
+          if (both) {
+            uint32_t o1[32];
+            tmem_ld32(to + D + c, o1);
+            tc_wait_ld();
 #pragma unroll
-            for (int x = 0; x < 32; x += 8) {
-              uint4 v;
-              v.x = pack_bf16x2(__uint_as_float(o[x]) * inv, __uint_as_float(o[x + 1]) * inv);
-              v.y = pack_bf16x2(__uint_as_float(o[x + 2]) * inv, __uint_as_float(o[x + 3]) * inv);
-              v.z = pack_bf16x2(__uint_as_float(o[x + 4]) * inv, __uint_as_float(o[x + 5]) * inv);
-              v.w = pack_bf16x2(__uint_as_float(o[x + 6]) * inv, __uint_as_float(o[x + 7]) * inv);
-              *reinterpret_cast<uint4*>(dst + c + x) = v;
+            for (int x = 0; x < 32; ++x)
+              if (f1 != 0.f) o[x] = __float_as_uint(fmaf(__uint_as_float(o1[x]), f1, __uint_as_float(o[x])));
+          }
+          if (t < valid) {
+            if (it.slot < 0) {
+#pragma unroll
+              for (int x = 0; x < 32; x += 8)
+                *reinterpret_cast<uint4*>(dst + c + x) =
+                    make_uint4(pack_bf16x2(__uint_as_float(o[x]), __uint_as_float(o[x + 1])),
+                               pack_bf16x2(__uint_as_float(o[x + 2]), __uint_as_float(o[x + 3])),
+                               pack_bf16x2(__uint_as_float(o[x + 4]), __uint_as_float(o[x + 5])),
+                               pack_bf16x2(__uint_as_float(o[x + 6]), __uint_as_float(o[x + 7])));
+            } else {
+#pragma unroll
+              for (int x = 0; x < 32; x += 4)
+                *reinterpret_cast<uint4*>(p.ws_o + slot_row * D + c + x) = make_uint4(o[x], o[x + 1], o[x + 2], o[x + 3]);
             }
-          } else {
-#pragma unroll
-            for (int x = 0; x < 32; x += 4)
-              *reinterpret_cast<uint4*>(p.ws_o + slot_row * D + c + x) = make_uint4(o[x], o[x + 1], o[x + 2], o[x + 3]);
           }
         }
+        if (it.slot >= 0 && t < valid) p.ws_ml[slot_row] = make_float2(ml, l);
       }
-      if (it.slot >= 0 && t < valid)
-        p.ws_ml[slot_row] = make_float2(any && m != -INFINITY ? m * p.scale_log2 : -INFINITY, any ? l : 0.f);
+      tc_fence_before();
+      if (both) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(merged);
+      }
     }
-    tc_fence_before();
   }
+  tc_fence_before();
   __syncthreads();
   if (warp == 8) {
     tc_fence_after();
-    tmem_dealloc(tmem, 512);
+    tmem_dealloc(*tmem_holder, 512);
   }
 }
 
@@ -565,25 +898,31 @@ __global__ void __launch_bounds__(kMergeWarps * 32) ragged_merge_kernel(const Ra
 }
 
 template <int D, bool Q8>
-int launch_ragged(const RagArgs& a, const RagShape& s, const void* k_pool, const void* v_pool, cudaStream_t st) {
+int launch_ragged(const RagArgs& a, const RagShape& s, const void* q, const void* k_pool, const void* v_pool, cudaStream_t st) {
   using C = RagCfg<D, Q8>;
   static bool done[64] = {};
   static std::mutex mu;
   MG_CUDA_TRY(mg_once_per_device(done, mu, [] {
     return cudaFuncSetAttribute(ragged_attn_kernel<D, Q8>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
   }));
-  CUtensorMap tk{}, tv{};
+  CUtensorMap tq{}, tk{}, tv{};
+  const CUtensorMapSwizzle sw = D >= 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
+  // Q as [rows][hq][D]: one box is a row tile, tokens times heads of a group, one row of shared memory each
+  int rc = mg_make_map_3d(&tq, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, q, {(uint64_t)D, (uint64_t)a.hq, (uint64_t)a.rows},
+                          {(uint64_t)D * 2, (uint64_t)a.hq * D * 2},
+                          {(uint32_t)C::kSlab / 2, (uint32_t)a.group, (uint32_t)a.tok_tile}, sw);
+  if (rc) return rc;
   if constexpr (!Q8) {
     const uint64_t rows = (uint64_t)a.num_blocks * a.hkv * 16;
     if (rows > 0x7fffffffull) return MG_ERR_UNSUPPORTED;
-    const CUtensorMapSwizzle sw = D >= 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
-    int rc = mg_make_map_2d(&tk, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, k_pool, D, rows, D * 2, C::kSlab / 2, 16, sw);
+    rc = mg_make_map_2d(&tk, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, k_pool, D, rows, D * 2, C::kSlab / 2, 16, sw);
     if (rc == MG_OK) rc = mg_make_map_2d(&tv, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, v_pool, D, rows, D * 2, C::kSlab / 2, 16, sw);
     if (rc) return rc;
   }
-  const int64_t ctas = s.max_list * a.hkv;
-  if (ctas > 0x7fffffff || a.hkv > 65535) return MG_ERR_UNSUPPORTED;
-  MG_CUDA_TRY(mg_launch(ragged_attn_kernel<D, Q8>, dim3((unsigned)ctas), dim3(C::kThreads), C::kSmem, st, 1, tk, tv, a));
+  const int64_t most = s.max_list * a.hkv;
+  if (most > 0x7fffffff || a.hkv > 65535) return MG_ERR_UNSUPPORTED;
+  const unsigned ctas = (unsigned)(most < mg_sm_count() ? most : mg_sm_count());
+  MG_CUDA_TRY(mg_launch(ragged_attn_kernel<D, Q8>, dim3(ctas), dim3(C::kThreads), C::kSmem, st, 1, tq, tk, tv, a));
   MG_CUDA_TRY(mg_launch(ragged_merge_kernel<D>, dim3((unsigned)s.max_merges, (unsigned)a.hkv, 8), dim3(kMergeWarps * 32),
                         0, st, 1, a));
   MG_LAUNCH_CHECK();
@@ -618,10 +957,10 @@ extern "C" int mg_ragged_attn(const void* q, int64_t rows, const void* k_pool, c
   if (!q || !k_pool || !v_pool || !block_tables || !work || !out || !workspace || workspace_bytes < need)
     return MG_ERR_INVALID_ARG;
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_pool) | reinterpret_cast<uintptr_t>(v_pool) |
-       reinterpret_cast<uintptr_t>(work) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(workspace)) & 15)
+       reinterpret_cast<uintptr_t>(k_scales) | reinterpret_cast<uintptr_t>(v_scales) | reinterpret_cast<uintptr_t>(work) |
+       reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(workspace)) & 15)
     return MG_ERR_INVALID_ARG;
   RagArgs a{};
-  a.q = static_cast<const __nv_bfloat16*>(q);
   a.rows = rows;
   a.num_blocks = num_blocks;
   a.tables = block_tables;
@@ -643,11 +982,13 @@ extern "C" int mg_ragged_attn(const void* q, int64_t rows, const void* k_pool, c
   a.out = static_cast<__nv_bfloat16*>(out);
   a.ws_o = static_cast<float*>(workspace);
   a.ws_ml = reinterpret_cast<float2*>(a.ws_o + (size_t)s.max_slots * hkv * 2 * kRows * d);
+  const int er = mg_error_words(&a.err_code, &a.err_info);
+  if (er) return er;
   cudaStream_t st = mg_stream(stream);
   if (q8) {
-    if (d == 32) return launch_ragged<32, true>(a, s, k_pool, v_pool, st);
-    return d == 64 ? launch_ragged<64, true>(a, s, k_pool, v_pool, st) : launch_ragged<128, true>(a, s, k_pool, v_pool, st);
+    if (d == 32) return launch_ragged<32, true>(a, s, q, k_pool, v_pool, st);
+    return d == 64 ? launch_ragged<64, true>(a, s, q, k_pool, v_pool, st) : launch_ragged<128, true>(a, s, q, k_pool, v_pool, st);
   }
-  if (d == 32) return launch_ragged<32, false>(a, s, k_pool, v_pool, st);
-  return d == 64 ? launch_ragged<64, false>(a, s, k_pool, v_pool, st) : launch_ragged<128, false>(a, s, k_pool, v_pool, st);
+  if (d == 32) return launch_ragged<32, false>(a, s, q, k_pool, v_pool, st);
+  return d == 64 ? launch_ragged<64, false>(a, s, q, k_pool, v_pool, st) : launch_ragged<128, false>(a, s, q, k_pool, v_pool, st);
 }

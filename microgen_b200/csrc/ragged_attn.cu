@@ -25,6 +25,8 @@
 // P is zero there, and 0 * V must be zero too: rows of V behind the item's last key are zeroed in the stage, and a
 // V row that some of a tile's rows may not see is looked over; where one holds an infinity or a NaN, that tile's
 // product is done by the softmax threads, over the keys each row sees.
+#include <type_traits>
+
 #include "ragged.cuh"
 
 namespace {
@@ -48,7 +50,8 @@ struct RagCfg {
   static constexpr int kCodeScales = kCodes + kCodeStages * kCodeBytes;
   static constexpr int kScales = kCodeScales + kCodeStages * kRows * 4;  // [ring][K 128 | V 128] fp32
   static constexpr int kMl = kScales + (Q8 ? kScaleRing * 2 * kRows * 4 : 0);  // [128] (maximum, sum)
-  static constexpr int kBars = kMl + kRows * 8;
+  static constexpr int kRedo = kMl + kRows * 8;                    // 32 words and one
+  static constexpr int kBars = kRedo + 256;
   static constexpr int kSmem = kBars + 512 + 1024;
   static_assert(kSmem <= 232448 - 64, "shared memory");
   static constexpr int kThreads = Q8 ? 512 : 384;
@@ -61,8 +64,6 @@ struct RagCfg {
   static constexpr uint32_t kIdescS = (1u << 4) | (1u << 7) | (1u << 10) | ((kRows >> 3) << 17) | ((kRows >> 4) << 24);
   static constexpr uint32_t kIdescO =
       (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((kRows >> 4) << 24);
-  // one in kPolyEvery pairs of exponentials is computed on the FMA pipe (0: none)
-  static constexpr int kPolyEvery = 0;
 };
 
 // Byte offset of the 16-byte chunk `c` (8 bf16) of row r in a swizzled tile.
@@ -117,6 +118,11 @@ __device__ __forceinline__ bool elect_one() {
   asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.b32 %0, 1, 0, q;\n\t}" : "=r"(p));
   return p != 0;
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 __device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
 
 // mbar_wait with its polls in one asm loop: 43 cycles where the phase is already over, 179 as a C++ loop.
@@ -134,6 +140,14 @@ __device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity, int whe
       : "memory");
   if (!ok) mg_record_error(MG_ERR_TIMEOUT, where);
   return ok != 0;
+}
+
+// tcgen05.wait::ld that the loaded registers pass through: nothing that uses them can be moved ahead of it.
+__device__ __forceinline__ void wait_ld8(uint32_t (&r)[8]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7])
+               :
+               : "memory");
 }
 
 template <int N>
@@ -164,27 +178,6 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
   uint64_t r;
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
-}
-
-// 2^x of a pair, x <= 127, on the FMA pipe: x = n + f with n the nearest integer (adding 1.5 * 2^23 leaves n in the low
-// mantissa bits), 2^f on [-1/2, 1/2] by a degree-4 polynomial fitted for the least relative error (2.7e-6, well
-// below the 2^-9 of rounding P to bf16), and n added to the exponent. Below 2^-126 the result is some tiny number.
-__device__ __forceinline__ uint64_t ex2_poly2(uint64_t x) {
-  float a, b;
-  unpair(x, a, b);
-  x = pair(fmaxf(a, -126.f), fmaxf(b, -126.f));
-  const uint64_t magic = pair(12582912.f, 12582912.f), minus = pair(-12582912.f, -12582912.f);
-  const uint64_t t = add2(x, magic);
-  const uint64_t f = fma2(add2(t, minus), pair(-1.f, -1.f), x);
-  uint64_t y = fma2(pair(0.009570100344717503f, 0.009570100344717503f), f, pair(0.05591785907745361f, 0.05591785907745361f));
-  y = fma2(y, f, pair(0.240247443318367f, 0.240247443318367f));
-  y = fma2(y, f, pair(0.6931217908859253f, 0.6931217908859253f));
-  y = fma2(y, f, pair(0.9999992847442627f, 0.9999992847442627f));
-  float ta, tb, ya, yb;
-  unpair(t, ta, tb);
-  unpair(y, ya, yb);
-  return pair(__int_as_float(__float_as_int(ya) + (__float_as_int(ta) << 23)),
-              __int_as_float(__float_as_int(yb) + (__float_as_int(tb) << 23)));
 }
 
 struct RagArgs {
@@ -226,6 +219,24 @@ __device__ __forceinline__ RagItem rag_item(const RagArgs& p, int index) {
   }
   return r;
 }
+// A CTA's way through its work: all of it, and (again) the pieces that have to be done over.
+constexpr int kRedoWords = 32;
+struct RagWalk {
+  int k, total, index;
+  RagItem it;
+  __device__ __forceinline__ void start(const RagArgs& p, int n, const volatile uint32_t* redo) {
+    k = -1;
+    total = n;
+    next(p, redo);
+  }
+  // redo: the pieces to do over, one bit each (the last bit stands for all behind it too), or null
+  __device__ __forceinline__ void next(const RagArgs& p, const volatile uint32_t* redo) {
+    do {
+      index = rag_index(++k, total);
+    } while (redo && index >= 0 && !(redo[min(k >> 5, kRedoWords - 1)] >> (k < 32 * kRedoWords ? k & 31 : 31) & 1u));
+    it = rag_item(p, index);
+  }
+};
 // The work of an item; one that does not fit this call's arrays (a plan for other sizes) has no tiles.
 __device__ __forceinline__ RagWork rag_work(const RagArgs& p, const RagItem& it, int index) {
   RagWork w;
@@ -255,6 +266,61 @@ __device__ __forceinline__ RagWork rag_work(const RagArgs& p, const RagItem& it,
   return w;
 }
 
+// Whether rows [r0, r1) of a V tile hold an infinity or a NaN (by the warps of a warpgroup, t = 0 .. 127; the answer is the
+// warp's). A bf16 infinity or NaN has all exponent bits set: adding one at the lowest of them carries out.
+template <int D>
+__device__ __noinline__ bool odd_rows(const uint8_t* v, int r0, int r1, int t) {
+  constexpr int kChunks = D / 8;
+  uint32_t acc = 0;
+  for (int x = r0 * kChunks + t; x < r1 * kChunks; x += 128) {
+    const uint4 q = *reinterpret_cast<const uint4*>(v + chunk_at<D>(x / kChunks, x % kChunks));
+    acc |= ((q.x & 0x7f807f80u) + 0x00800080u) | ((q.y & 0x7f807f80u) + 0x00800080u) |
+           ((q.z & 0x7f807f80u) + 0x00800080u) | ((q.w & 0x7f807f80u) + 0x00800080u);
+  }
+  return __any_sync(0xffffffffu, (acc & 0x80008000u) != 0);
+}
+
+// O += P V over the keys 0 .. see of a tile that the thread's row sees, from the stage, in the tensor cores' place. ts, to:
+// the warp's tensor-memory addresses of P and O; `more`: something is in O already. (Not inlined, like odd_rows: in the
+// loop's body their registers and code cost every call 5 % and serve none but those with an infinity or NaN in V.)
+template <int D>
+__device__ __noinline__ void values_by_hand(const uint8_t* v, uint32_t ts, uint32_t to, int see, bool more) {
+#pragma unroll 1
+  for (int c = 0; c < D; c += 8) {
+    float o[8] = {};
+    uint32_t x8[8];
+    if (more) {
+      tmem_ld8(to + c, x8);
+      wait_ld8(x8);
+#pragma unroll
+      for (int x = 0; x < 8; ++x) o[x] = __uint_as_float(x8[x]);
+    }
+#pragma unroll 1
+    for (int q = 0; q < kRows; q += 16) {
+      uint32_t pr[8];
+      tmem_ld8(ts + q / 2, pr);
+      wait_ld8(pr);
+#pragma unroll
+      for (int y = 0; y < 16; ++y) {
+        const float pv = y & 1 ? bf16hi(pr[y / 2]) : bf16lo(pr[y / 2]);
+        if (q + y <= see) {
+          const uint4 x4 = *reinterpret_cast<const uint4*>(v + chunk_at<D>(q + y, c / 8));
+          const uint32_t e[4] = {x4.x, x4.y, x4.z, x4.w};
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            o[2 * x] = fmaf(pv, bf16lo(e[x]), o[2 * x]);
+            o[2 * x + 1] = fmaf(pv, bf16hi(e[x]), o[2 * x + 1]);
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int x = 0; x < 8; ++x) x8[x] = __float_as_uint(o[x]);
+    tmem_st8(to + c, x8);
+  }
+  tc_wait_st();
+}
+
 template <int D, bool Q8>
 __global__ void __launch_bounds__(RagCfg<D, Q8>::kThreads, 1)
     ragged_attn_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
@@ -273,16 +339,20 @@ __global__ void __launch_bounds__(RagCfg<D, Q8>::kThreads, 1)
   uint64_t* sfull = qfree + 2;     // [2] scores are in tensor memory (and the warpgroup's earlier P V is done)
   uint64_t* pready = sfull + 2;    // [2] probabilities are
   uint64_t* ofull = pready + 2;    // [2] the item's output is complete
-  uint64_t* looked = ofull + 2;    // [2] every warp has looked over a masked tile's V rows
+  uint64_t* looked = ofull + 2;    // [2] every warp has looked over a masked tile's V rows (second pass)
   uint64_t* mlready = looked + 2;  // the second warpgroup's (maximum, sum) are in shared memory
   uint64_t* merged = mlready + 1;  // ... and its output has been read
   uint64_t* drained = merged + 1;
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(drained + 1);
-  int* skip = reinterpret_cast<int*>(tmem_holder + 1);  // [2] the softmax threads did this tile's P V themselves
-  int* odd_v = skip + 2;           // [2] an infinity or NaN was found among V rows that some row may not see
+  volatile int* skip = reinterpret_cast<volatile int*>(tmem_holder + 1);  // [2] the softmax threads did a tile's P V
+  volatile int* odd_v = skip + 2;  // [2] an infinity or NaN was found among V rows that some row may not see
+  volatile uint32_t* redo = reinterpret_cast<volatile uint32_t*>(smem + C::kRedo);  // pieces for a second pass ...
+  volatile uint32_t* redo_any = redo + kRedoWords;                                   // ... and whether there are any
+  auto block_barrier = [] { asm volatile("bar.sync 1, %0;" ::"n"(C::kThreads) : "memory"); };
 
   griddep_launch();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x <= kRedoWords) redo[threadIdx.x] = 0;
   if (threadIdx.x == 0) {
     mg_set_error_words(p.err_code, p.err_info);
     for (int s = 0; s < NS; ++s) {
@@ -300,7 +370,8 @@ __global__ void __launch_bounds__(RagCfg<D, Q8>::kThreads, 1)
       mbar_init(&pready[w], 4);
       mbar_init(&ofull[w], 1);
       mbar_init(&looked[w], 4);
-      skip[w] = odd_v[w] = 0;
+      skip[w] = 0;
+      odd_v[w] = 0;
     }
     mbar_init(mlready, 4);
     mbar_init(merged, 4);
@@ -321,93 +392,97 @@ __global__ void __launch_bounds__(RagCfg<D, Q8>::kThreads, 1)
   if (warp >= 8) {
     regs_dec<C::kOtherRegs>();
     bool ok = true;
-    int index = rag_index(0, total);
-    RagItem next = rag_item(p, index);
+    RagWalk walk;
     if (warp == 8) {
       // ---------------- tensor-core issue ----------------
       const uint32_t sq = smem_u32(smem), sr = smem_u32(smem + C::kRing);
       const uint64_t q_desc = rag_desc<D>(sq, 16), k_desc = rag_desc<D>(sr, 16), v_desc = rag_desc<D>(sr, C::kSlabBytes);
       int base = 0;
       uint32_t pp = 0, pq = 0;  // phase bits of pready and qfull, one per row tile
-      for (int k = 0; index >= 0 && ok; ++k) {
-        const RagWork wk = rag_work(p, next, index);
-        index = rag_index(k + 1, total);
-        next = rag_item(p, index);
-        const int tiles = uniform(wk.tiles), n0 = uniform(wk.n0), n1 = uniform(wk.n1);
-        const bool dual = uniform(wk.dual) != 0;
-        // S_w = Q_w K_j^T (in a branch of one thread)
-        auto scores = [&](int w, int j) {
-          const uint64_t a = q_desc + (uint64_t)(w * (C::kTileBytes >> 4));
-          const uint64_t b = k_desc + (uint64_t)(((base + 2 * j) % NS) * (C::kTileBytes >> 4));
+      for (int pass = 0; pass < 2; ++pass) {
+        walk.start(p, total, pass ? redo : nullptr);
+        while (walk.index >= 0 && ok) {
+          const RagWork wk = rag_work(p, walk.it, walk.index);
+          walk.next(p, pass ? redo : nullptr);
+          const int tiles = uniform(wk.tiles), n0 = uniform(wk.n0), n1 = uniform(wk.n1);
+          const bool dual = uniform(wk.dual) != 0;
+          // S_w = Q_w K_j^T (in a branch of one thread)
+          auto scores = [&](int w, int j) {
+            const uint64_t a = q_desc + (uint64_t)(w * (C::kTileBytes >> 4));
+            const uint64_t b = k_desc + (uint64_t)(((base + 2 * j) % NS) * (C::kTileBytes >> 4));
 #pragma unroll
-          for (int x = 0; x < D / 16; ++x) {
-            const uint64_t off = (uint64_t)(((x * 32 / C::kSlab) * C::kSlabBytes + (x * 32) % C::kSlab) >> 4);
-            tc_mma_ss((uint32_t)(w * kRows), a + off, b + off, C::kIdescS, x > 0);
-          }
-          tc_commit(&sfull[w]);
-        };
-        auto await_k = [&](int j) {
-          const int i = base + 2 * j;
-          ok = ok && bar_wait(&full[i % NS], (i / NS) & 1, 515);
-          tc_fence_after();
-        };
-        const int step = dual ? 2 : 1;
-#pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          const int n = w ? n1 : n0;
-          if (n == 0 || !ok) continue;
-          ok = bar_wait(&qfull[w], (pq >> w) & 1, 514);
-          pq ^= 1u << w;
-          const int j = dual ? w : 0;
-          if (dual || w == 0 || n0 == 0) await_k(j);
-          if (!ok) break;
-          if (elect_one()) {
-            scores(w, j);
-            if (n == 1) tc_commit(&qfree[w]);
-            if (dual || w == 1) tc_commit(&empty[(base + 2 * j) % NS]);
-          }
-          __syncwarp();
-        }
-        for (int j = 0; j < tiles && ok; ++j) {
-          const int iv = base + 2 * j + 1, jn = j + step;
-          const uint64_t v = v_desc + (uint64_t)((iv % NS) * (C::kTileBytes >> 4));
-          ok = bar_wait(&full[iv % NS], (iv / NS) & 1, 516);
-          bool k_here = false;
+            for (int x = 0; x < D / 16; ++x) {
+              const uint64_t off = (uint64_t)(((x * 32 / C::kSlab) * C::kSlabBytes + (x * 32) % C::kSlab) >> 4);
+              tc_mma_ss((uint32_t)(w * kRows), a + off, b + off, C::kIdescS, x > 0);
+            }
+            tc_commit(&sfull[w]);
+          };
+          auto await_k = [&](int j) {
+            const int i = base + 2 * j;
+            ok = ok && bar_wait(&full[i % NS], (i / NS) & 1, 515);
+            tc_fence_after();
+          };
+          const int step = dual ? 2 : 1;
 #pragma unroll
           for (int w = 0; w < 2; ++w) {
-            const int last = dual ? tiles : (w ? n1 : n0);
-            if (!ok || (dual ? w != (j & 1) : j >= last)) continue;
-            ok = bar_wait(&pready[w], (pp >> w) & 1, 517);
+            const int n = w ? n1 : n0;
+            if (n == 0 || !ok) continue;
+            ok = bar_wait(&qfull[w], (pq >> w) & 1, 514);
+            pq ^= 1u << w;
+            const int j = dual ? w : 0;
+            if (dual || w == 0 || n0 == 0) await_k(j);
             if (!ok) break;
-            pp ^= 1u << w;
-            tc_fence_after();
-            const bool by_hand = !Q8 && uniform(*(volatile int*)&skip[w]) != 0;
             if (elect_one()) {
-              if (!by_hand) {
-                const uint32_t more = j >= step;  // something is in O already
-#pragma unroll
-                for (int x = 0; x < kRows / 16; ++x)  // 16 keys a step: 16 rows of V
-                  tc_mma_ts(C::kO + (uint32_t)(w * D), (uint32_t)(w * kRows + x * 8),
-                            v + (uint64_t)((x * 16 * C::kSlab) >> 4), C::kIdescO, x > 0 ? 1u : more);
-              }
-              if (dual || w == 1) tc_commit(&empty[iv % NS]);
-              if (jn >= last) tc_commit(&ofull[w]);
+              scores(w, j);
+              if (n == 1) tc_commit(&qfree[w]);
+              if (dual || w == 1) tc_commit(&empty[(base + 2 * j) % NS]);
             }
             __syncwarp();
-            if (jn < last) {
-              if (!k_here) await_k(jn);
-              k_here = true;
+          }
+          for (int j = 0; j < tiles && ok; ++j) {
+            const int iv = base + 2 * j + 1, jn = j + step;
+            const uint64_t v = v_desc + (uint64_t)((iv % NS) * (C::kTileBytes >> 4));
+            ok = bar_wait(&full[iv % NS], (iv / NS) & 1, 516);
+            bool k_here = false;
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+              const int last = dual ? tiles : (w ? n1 : n0);
+              if (!ok || (dual ? w != (j & 1) : j >= last)) continue;
+              ok = bar_wait(&pready[w], (pp >> w) & 1, 517);
               if (!ok) break;
+              pp ^= 1u << w;
+              tc_fence_after();
+              const bool by_hand = !Q8 && pass && uniform(skip[w]) != 0;
               if (elect_one()) {
-                scores(w, jn);
-                if (jn + step >= last) tc_commit(&qfree[w]);
-                if (dual || w == 1) tc_commit(&empty[(base + 2 * jn) % NS]);
+                if (!by_hand) {
+                  const uint32_t more = j >= step;  // something is in O already
+#pragma unroll
+                  for (int x = 0; x < kRows / 16; ++x)  // 16 keys a step: 16 rows of V
+                    tc_mma_ts(C::kO + (uint32_t)(w * D), (uint32_t)(w * kRows + x * 8),
+                              v + (uint64_t)((x * 16 * C::kSlab) >> 4), C::kIdescO, x > 0 ? 1u : more);
+                }
+                if (dual || w == 1) tc_commit(&empty[iv % NS]);
+                if (jn >= last) tc_commit(&ofull[w]);
               }
               __syncwarp();
+              if (jn < last) {
+                if (!k_here) await_k(jn);
+                k_here = true;
+                if (!ok) break;
+                if (elect_one()) {
+                  scores(w, jn);
+                  if (jn + step >= last) tc_commit(&qfree[w]);
+                  if (dual || w == 1) tc_commit(&empty[(base + 2 * jn) % NS]);
+                }
+                __syncwarp();
+              }
             }
           }
+          base += 2 * tiles;
         }
-        base += 2 * tiles;
+        if (Q8 || pass) break;
+        block_barrier();
+        if (!*redo_any) break;
       }
       if (elect_one()) tc_commit(drained);
       __syncwarp();
@@ -418,61 +493,66 @@ __global__ void __launch_bounds__(RagCfg<D, Q8>::kThreads, 1)
       // tile's b-th block id, fetched a tile ahead; one lane starts the copies
       int i = 0;
       const int blk = lane & 7;
-      for (int k = 0; index >= 0 && ok; ++k) {
-        const RagWork wk = rag_work(p, next, index);
-        if (wk.it.n_tok == 0) mg_record_error(MG_ERR_DEVICE, 510);
-        index = rag_index(k + 1, total);
-        next = rag_item(p, index);
-        const int32_t* table = p.tables + (int64_t)wk.it.seq * p.max_blocks;
-        const int blocks = (wk.it.kv_len + 15) >> 4;
-        int b0 = wk.it.kt0 * 8;
-        int32_t id_next = wk.tiles > 0 && b0 + blk < blocks ? table[b0 + blk] : 0;
-        for (int j = 0; j < wk.tiles && ok; ++j, b0 += 8) {
-          const int nb = min(8, blocks - b0);
-          const int32_t id = id_next;
-          const bool good = id >= 0 && id < p.num_blocks;
-          if (blk < nb && !good) mg_record_error(MG_ERR_DEVICE, 511);
-          if (b0 + 8 + blk < blocks) id_next = table[b0 + 8 + blk];
+      for (int pass = 0; pass < 2; ++pass) {
+        walk.start(p, total, pass ? redo : nullptr);
+        while (walk.index >= 0 && ok) {
+          const RagWork wk = rag_work(p, walk.it, walk.index);
+          if (wk.it.n_tok == 0) mg_record_error(MG_ERR_DEVICE, 510);
+          walk.next(p, pass ? redo : nullptr);
+          const int32_t* table = p.tables + (int64_t)wk.it.seq * p.max_blocks;
+          const int blocks = (wk.it.kv_len + 15) >> 4;
+          int b0 = wk.it.kt0 * 8;
+          int32_t id_next = wk.tiles > 0 && b0 + blk < blocks ? table[b0 + blk] : 0;
+          for (int j = 0; j < wk.tiles && ok; ++j, b0 += 8) {
+            const int nb = min(8, blocks - b0);
+            const int32_t id = id_next;
+            const bool good = id >= 0 && id < p.num_blocks;
+            if (blk < nb && !good) mg_record_error(MG_ERR_DEVICE, 511);
+            if (b0 + 8 + blk < blocks) id_next = table[b0 + 8 + blk];
 #pragma unroll
-          for (int kv = 0; kv < 2; ++kv, ++i) {
-            if constexpr (Q8) {
-              const int s = i % NC;
-              if (i >= NC) ok = ok && bar_wait(&cempty[s], ((i / NC) - 1) & 1, 512);
-              if (!ok) break;
-              // a block that is not in the pool is read as the pool's first (its error has been recorded)
-              const int row = (good ? id : 0) * p.hkv + wk.head;
-              if (elect_one()) mbar_arrive_expect_tx(&cfull[s], (uint32_t)(nb * 16 * (D + 4)));
+            for (int kv = 0; kv < 2; ++kv, ++i) {
+              if constexpr (Q8) {
+                const int s = i % NC;
+                if (i >= NC) ok = ok && bar_wait(&cempty[s], ((i / NC) - 1) & 1, 512);
+                if (!ok) break;
+                // a block that is not in the pool is read as the pool's first (its error has been recorded)
+                const int row = (good ? id : 0) * p.hkv + wk.head;
+                if (elect_one()) mbar_arrive_expect_tx(&cfull[s], (uint32_t)(nb * 16 * (D + 4)));
 #pragma unroll
-              for (int y = 0; y < 8; ++y) {
-                const int64_t r = (int64_t)__shfl_sync(0xffffffffu, row, y) * 16;
-                if (y < nb && elect_one()) {
-                  bulk_load_smem(smem + C::kCodes + s * C::kCodeBytes + y * 16 * D, (kv ? p.v8 : p.k8) + r * D, 16 * D,
-                                 &cfull[s]);
-                  bulk_load_smem(smem + C::kCodeScales + s * kRows * 4 + y * 64, (kv ? p.vs : p.ks) + r, 64, &cfull[s]);
+                for (int y = 0; y < 8; ++y) {
+                  const int64_t r = (int64_t)__shfl_sync(0xffffffffu, row, y) * 16;
+                  if (y < nb && elect_one()) {
+                    bulk_load_smem(smem + C::kCodes + s * C::kCodeBytes + y * 16 * D, (kv ? p.v8 : p.k8) + r * D, 16 * D,
+                                   &cfull[s]);
+                    bulk_load_smem(smem + C::kCodeScales + s * kRows * 4 + y * 64, (kv ? p.vs : p.ks) + r, 64, &cfull[s]);
+                  }
+                  __syncwarp();
                 }
-                __syncwarp();
-              }
-            } else {
-              const int s = i % NS;
-              if (i >= NS) ok = ok && bar_wait(&empty[s], ((i / NS) - 1) & 1, 512);
-              if (!ok) break;
-              // (a block that is not in the pool is read behind its end: as zeros)
-              const int row = (int)(good ? (id * p.hkv + wk.head) * 16 : p.num_blocks * p.hkv * 16);
-              if (elect_one()) mbar_arrive_expect_tx(&full[s], (uint32_t)(nb * 16 * D * 2));
+              } else {
+                const int s = i % NS;
+                if (i >= NS) ok = ok && bar_wait(&empty[s], ((i / NS) - 1) & 1, 512);
+                if (!ok) break;
+                // (a block that is not in the pool is read behind its end: as zeros)
+                const int row = (int)(good ? (id * p.hkv + wk.head) * 16 : p.num_blocks * p.hkv * 16);
+                if (elect_one()) mbar_arrive_expect_tx(&full[s], (uint32_t)(nb * 16 * D * 2));
 #pragma unroll
-              for (int y = 0; y < 8; ++y) {
-                const int r = __shfl_sync(0xffffffffu, row, y);
-                if (y < nb && elect_one()) {
+                for (int y = 0; y < 8; ++y) {
+                  const int r = __shfl_sync(0xffffffffu, row, y);
+                  if (y < nb && elect_one()) {
 #pragma unroll
-                  for (int x = 0; x < C::kSlabs; ++x)
-                    tma_load_2d(smem + C::kRing + s * C::kTileBytes + x * C::kSlabBytes + y * 16 * C::kSlab, kv ? &tv : &tk,
-                                &full[s], x * (C::kSlab / 2), r);
+                    for (int x = 0; x < C::kSlabs; ++x)
+                      tma_load_2d(smem + C::kRing + s * C::kTileBytes + x * C::kSlabBytes + y * 16 * C::kSlab, kv ? &tv : &tk,
+                                  &full[s], x * (C::kSlab / 2), r);
+                  }
+                  __syncwarp();
                 }
-                __syncwarp();
               }
             }
           }
         }
+        if (Q8 || pass) break;
+        block_barrier();
+        if (!*redo_any) break;
       }
       // the loads that were started have landed before this CTA's memory goes to another
       if constexpr (Q8) {
@@ -483,29 +563,36 @@ __global__ void __launch_bounds__(RagCfg<D, Q8>::kThreads, 1)
     } else if (warp == 10) {
       // ---------------- Q loads: a row tile's tokens x heads of the group, as soon as the products before are done ------
       int c0 = 0, c1 = 0;  // loads so far
-      for (int k = 0; index >= 0 && ok; ++k) {
-        const RagWork wk = rag_work(p, next, index);
-        index = rag_index(k + 1, total);
-        next = rag_item(p, index);
+      for (int pass = 0; pass < 2; ++pass) {
+        walk.start(p, total, pass ? redo : nullptr);
+        while (walk.index >= 0 && ok) {
+          const RagWork wk = rag_work(p, walk.it, walk.index);
+          walk.next(p, pass ? redo : nullptr);
 #pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          int& c = w ? c1 : c0;
-          if ((w ? wk.n1 : wk.n0) == 0 || !ok) continue;
-          if (c > 0) ok = bar_wait(&qfree[w], (c - 1) & 1, 524);
-          if (!ok) break;
-          ++c;
-          if (elect_one()) {
-            mbar_arrive_expect_tx(&qfull[w], (uint32_t)(C::kSlabs * p.tok_tile * p.group * C::kSlab));
+          for (int w = 0; w < 2; ++w) {
+            int& c = w ? c1 : c0;
+            if ((w ? wk.n1 : wk.n0) == 0 || !ok) continue;
+            if (c > 0) ok = bar_wait(&qfree[w], (c - 1) & 1, 524);
+            if (!ok) break;
+            ++c;
+            if (elect_one()) {
+              mbar_arrive_expect_tx(&qfull[w], (uint32_t)(C::kSlabs * p.tok_tile * p.group * C::kSlab));
 #pragma unroll
-            for (int s = 0; s < C::kSlabs; ++s)
-              tma_load_3d(smem + w * C::kTileBytes + s * C::kSlabBytes, &tq, &qfull[w], s * (C::kSlab / 2),
-                          wk.head * p.group, wk.it.row0 + (wk.dual ? 0 : w * p.tok_tile));
+              for (int s = 0; s < C::kSlabs; ++s)
+                tma_load_3d(smem + w * C::kTileBytes + s * C::kSlabBytes, &tq, &qfull[w], s * (C::kSlab / 2),
+                            wk.head * p.group, wk.it.row0 + (wk.dual ? 0 : w * p.tok_tile));
+            }
+            __syncwarp();
           }
-          __syncwarp();
         }
+        if (Q8 || pass) break;
+        block_barrier();
+        if (!*redo_any) break;
       }
       if (c0 > 0) bar_wait(&qfull[0], (c0 - 1) & 1, 525);
       if (c1 > 0) bar_wait(&qfull[1], (c1 - 1) & 1, 525);
+    } else if (!Q8 && warp == 11) {
+      block_barrier();  // (the passes' barrier; this warp has no part in either)
     } else if (Q8 && warp >= 12) {
       // ---------------- int8 codes -> bf16 tiles, swizzled ----------------
       const int t = threadIdx.x - 12 * 32;
@@ -513,43 +600,48 @@ __global__ void __launch_bounds__(RagCfg<D, Q8>::kThreads, 1)
       constexpr int kParts = D / 16;              // 16-byte pieces of a vector of codes
       constexpr int kPer = kRows * kParts / 128;  // pieces per thread and tile
       int i = 0, tile = 0;
-      for (int k = 0; index >= 0 && ok; ++k) {
-        const RagWork wk = rag_work(p, next, index);
-        index = rag_index(k + 1, total);
-        next = rag_item(p, index);
-        for (int j = 0; j < wk.tiles && ok; ++j, ++tile) {
-          const int keys = wk.it.kv_len - (wk.it.kt0 + j) * kRows;  // of the tile, where fewer than 128
+      for (int pass = 0; pass < 2; ++pass) {
+        walk.start(p, total, pass ? redo : nullptr);
+        while (walk.index >= 0 && ok) {
+          const RagWork wk = rag_work(p, walk.it, walk.index);
+          walk.next(p, pass ? redo : nullptr);
+          for (int j = 0; j < wk.tiles && ok; ++j, ++tile) {
+            const int keys = wk.it.kv_len - (wk.it.kt0 + j) * kRows;  // of the tile, where fewer than 128
 #pragma unroll 1
-          for (int kv = 0; kv < 2; ++kv, ++i) {
-            const int s = i % NS, sc = i % NC;
-            ok = ok && bar_wait(&cfull[sc], (i / NC) & 1, 526);
-            if (i >= NS) ok = ok && bar_wait(&empty[s], ((i / NS) - 1) & 1, 527);
-            if (!ok) break;
-            const uint8_t* src = smem + C::kCodes + sc * C::kCodeBytes;
-            uint8_t* dst = smem + C::kRing + s * C::kTileBytes;
+            for (int kv = 0; kv < 2; ++kv, ++i) {
+              const int s = i % NS, sc = i % NC;
+              ok = ok && bar_wait(&cfull[sc], (i / NC) & 1, 526);
+              if (i >= NS) ok = ok && bar_wait(&empty[s], ((i / NS) - 1) & 1, 527);
+              if (!ok) break;
+              const uint8_t* src = smem + C::kCodes + sc * C::kCodeBytes;
+              uint8_t* dst = smem + C::kRing + s * C::kTileBytes;
 #pragma unroll
-            for (int x = 0; x < kPer; ++x) {
-              const int piece = x * 128 + t, r = piece / kParts, q = (piece % kParts) * 2;
-              uint4 c = make_uint4(0, 0, 0, 0);
-              if (r < keys) c = *reinterpret_cast<const uint4*>(src + piece * 16);
-              uint4 lo, hi;
-              i8x4_to_bf16x4(c.x, lo.x, lo.y);
-              i8x4_to_bf16x4(c.y, lo.z, lo.w);
-              i8x4_to_bf16x4(c.z, hi.x, hi.y);
-              i8x4_to_bf16x4(c.w, hi.z, hi.w);
-              *reinterpret_cast<uint4*>(dst + chunk_at<D>(r, q)) = lo;
-              *reinterpret_cast<uint4*>(dst + chunk_at<D>(r, q + 1)) = hi;
-            }
-            scales[(tile % C::kScaleRing) * 2 * kRows + kv * kRows + t] =
-                t < keys ? reinterpret_cast<const float*>(smem + C::kCodeScales)[sc * kRows + t] : 0.f;
-            fence_async_smem();
-            __syncwarp();
-            if (lane == 0) {
-              mbar_arrive(&cempty[sc]);
-              mbar_arrive(&full[s]);
+              for (int x = 0; x < kPer; ++x) {
+                const int piece = x * 128 + t, r = piece / kParts, q = (piece % kParts) * 2;
+                uint4 c = make_uint4(0, 0, 0, 0);
+                if (r < keys) c = *reinterpret_cast<const uint4*>(src + piece * 16);
+                uint4 lo, hi;
+                i8x4_to_bf16x4(c.x, lo.x, lo.y);
+                i8x4_to_bf16x4(c.y, lo.z, lo.w);
+                i8x4_to_bf16x4(c.z, hi.x, hi.y);
+                i8x4_to_bf16x4(c.w, hi.z, hi.w);
+                *reinterpret_cast<uint4*>(dst + chunk_at<D>(r, q)) = lo;
+                *reinterpret_cast<uint4*>(dst + chunk_at<D>(r, q + 1)) = hi;
+              }
+              scales[(tile % C::kScaleRing) * 2 * kRows + kv * kRows + t] =
+                  t < keys ? reinterpret_cast<const float*>(smem + C::kCodeScales)[sc * kRows + t] : 0.f;
+              fence_async_smem();
+              __syncwarp();
+              if (lane == 0) {
+                mbar_arrive(&cempty[sc]);
+                mbar_arrive(&full[s]);
+              }
             }
           }
         }
+        if (Q8 || pass) break;
+        block_barrier();
+        if (!*redo_any) break;
       }
     }
   } else {
@@ -564,290 +656,246 @@ __global__ void __launch_bounds__(RagCfg<D, Q8>::kThreads, 1)
     const uint64_t scale2 = pair(p.scale_log2, p.scale_log2);
     bool ok = true;
     int base = 0, cs = 0, co = 0, looks = 0, duals = 0, tile0 = 0;
-    int index = rag_index(0, total);
-    RagItem next = rag_item(p, index);
-    for (int k = 0; index >= 0 && ok; ++k) {
-      const RagWork wk = rag_work(p, next, index);
-      index = rag_index(k + 1, total);
-      next = rag_item(p, index);
-      const RagItem& it = wk.it;
-      const int tok0 = wk.dual ? 0 : w * p.tok_tile;
-      const int valid = max(0, min(p.tok_tile, it.n_tok - tok0)) * p.group;
-      const int first_pos = it.pos0 + tok0, my_pos = first_pos + my_tok;
-      const bool warp_on = (warp & 3) * 32 < valid;
-      const int n = w ? wk.n1 : wk.n0;
-      float m = -INFINITY;  // the maximum in use, in score units
-      uint64_t l2 = 0;      // the sum, in two halves
-      for (int i = 0; i < n && ok; ++i) {
-        const int j = wk.dual ? 2 * i + w : i;
-        const int key0 = (it.kt0 + j) * kRows;
-        ok = bar_wait(&sfull[w], cs++ & 1, 520);
-        if (!ok) break;
-        tc_fence_after();
-        const bool masked = key0 + kRows - 1 > first_pos;  // some row of the tile does not see all its keys
-        bool by_hand = false;
-        if constexpr (Q8) {  // the values' scales come with V
-          const int iv = base + 2 * j + 1;
-          ok = bar_wait(&full[iv % NS], (iv / NS) & 1, 521);
+    RagWalk walk;
+    // (a function of its own for the second pass: what only that does would cost the first one registers, 5 % of its time)
+    auto softmax_pass = [&](auto again_tag) {
+      constexpr bool kAgain = decltype(again_tag)::value;
+      walk.start(p, total, kAgain ? redo : nullptr);
+      while (walk.index >= 0 && ok) {
+        const RagWork wk = rag_work(p, walk.it, walk.index);
+        const int piece = walk.k;
+        walk.next(p, kAgain ? redo : nullptr);
+        const RagItem& it = wk.it;
+        const int tok0 = wk.dual ? 0 : w * p.tok_tile;
+        const int valid = max(0, min(p.tok_tile, it.n_tok - tok0)) * p.group;
+        const int first_pos = it.pos0 + tok0, my_pos = first_pos + my_tok;
+        const bool warp_on = (warp & 3) * 32 < valid;
+        const int n = w ? wk.n1 : wk.n0;
+        if (kAgain && t == 0) odd_v[w] = 0;
+        float m = -INFINITY;  // the maximum in use, in score units
+        uint64_t l2 = 0;      // the sum, in two halves
+        for (int i = 0; i < n && ok; ++i) {
+          const int j = wk.dual ? 2 * i + w : i;
+          const int key0 = (it.kt0 + j) * kRows;
+          ok = bar_wait(&sfull[w], cs++ & 1, 520);
           if (!ok) break;
-        } else {
-          if (i == 0 && t == 0) *(volatile int*)&odd_v[w] = 0;
-          if (masked) {
-            // V rows that some row may not see: zero those behind the item's keys, look the others over
+          tc_fence_after();
+          const bool masked = key0 + kRows - 1 > first_pos;  // some row of the tile does not see all its keys
+          bool by_hand = false;
+          if constexpr (Q8) {  // the values' scales come with V
+            const int iv = base + 2 * j + 1;
+            ok = bar_wait(&full[iv % NS], (iv / NS) & 1, 521);
+            if (!ok) break;
+          } else {
             const int iv = base + 2 * j + 1, sv = iv % NS;
-            ok = bar_wait(&full[sv], (iv / NS) & 1, 521);
-            if (!ok) break;
-            uint8_t* v = smem + C::kRing + sv * C::kTileBytes;
-            const int r_first = max(0, first_pos + 1 - key0), r_end = min(kRows, it.kv_len - key0);
-            // (a bf16 infinity or NaN has all exponent bits set: adding one at the lowest of them carries out)
-            uint32_t acc = 0;
-            constexpr int kChunks = D / 8, kBatch = 4;
-            for (int x0 = r_first * kChunks + t; x0 < kRows * kChunks; x0 += 128 * kBatch) {
-              uint4 q[kBatch];
-#pragma unroll
-              for (int y = 0; y < kBatch; ++y) {
-                const int x = x0 + y * 128;
-                q[y] = make_uint4(0, 0, 0, 0);
-                if (x < r_end * kChunks) q[y] = *reinterpret_cast<const uint4*>(v + chunk_at<D>(x / kChunks, x % kChunks));
-              }
-#pragma unroll
-              for (int y = 0; y < kBatch; ++y) {
-                const int x = x0 + y * 128;
-                if (x >= r_end * kChunks && x < kRows * kChunks)
-                  *reinterpret_cast<uint4*>(v + chunk_at<D>(x / kChunks, x % kChunks)) = make_uint4(0, 0, 0, 0);
-                acc |= ((q[y].x & 0x7f807f80u) + 0x00800080u) | ((q[y].y & 0x7f807f80u) + 0x00800080u) |
-                       ((q[y].z & 0x7f807f80u) + 0x00800080u) | ((q[y].w & 0x7f807f80u) + 0x00800080u);
-              }
-            }
-            bool odd = (acc & 0x80008000u) != 0;
-            fence_async_smem();
-            // (any thread's finding is every thread's; once found it holds for the item's later tiles too)
-            odd = __any_sync(0xffffffffu, odd);
-            if (lane == 0) {
-              if (odd) *(volatile int*)&odd_v[w] = 1;
-              mbar_arrive(&looked[w]);
-            }
-            ok = bar_wait(&looked[w], looks & 1, 523);
-            ++looks;
-            if (!ok) break;
-            by_hand = *(volatile int*)&odd_v[w] != 0;
-          }
-        }
-        if (warp_on) {
-          float s[kRows];
-#pragma unroll
-          for (int c = 0; c < 4; ++c) tmem_ld32(ts + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&s[c * 32]));
-          tc_wait_ld();
-          const float* sc = reinterpret_cast<const float*>(smem + C::kScales) + ((tile0 + j) % C::kScaleRing) * 2 * kRows;
-          if constexpr (Q8) {
-#pragma unroll
-            for (int c = 0; c < kRows; c += 4) {
-              const float4 f = *reinterpret_cast<const float4*>(sc + c);
-              s[c] *= f.x, s[c + 1] *= f.y, s[c + 2] *= f.z, s[c + 3] *= f.w;
-            }
-          }
-          const int see = my_pos - key0;  // keys 0 .. see of the tile are this row's
-          if (masked) {
-#pragma unroll
-            for (int c = 0; c < kRows; ++c) s[c] = c <= see ? s[c] : -INFINITY;
-          }
-          float mx[8];
-#pragma unroll
-          for (int c = 0; c < 8; ++c) mx[c] = fmaxf(s[c], s[c + 8]);
-#pragma unroll
-          for (int c = 16; c < kRows; c += 16) {
-#pragma unroll
-            for (int x = 0; x < 8; ++x) mx[x] = fmaxf(fmaxf(mx[x], s[c + x]), s[c + 8 + x]);
-          }
-          float m_new = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7])));
-          m_new = fmaxf(m, m_new);
-          const bool grow = m == -INFINITY || (m_new - m) * p.scale_log2 > 8.f;
-          if (!grow) m_new = m;
-          if (i > 0 && __any_sync(0xffffffffu, grow)) {
-            const float f = m == -INFINITY ? 0.f : ex2((m - m_new) * p.scale_log2);
-            l2 = mul2(l2, pair(f, f));
-#pragma unroll 1
-            for (int c = 0; c < D; c += 32) {
-              uint32_t o[32];
-              tmem_ld32(to + c, o);
-              tc_wait_ld();
-#pragma unroll
-              for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
-              tmem_st32(to + c, o);
-            }
-          }
-          m = m_new;
-          const float off = m == -INFINITY ? 0.f : -m * p.scale_log2;
-          const uint64_t off2 = pair(off, off);
-          uint64_t sum[2] = {l2, 0};
-#pragma unroll
-          for (int h = 0; h < 4; ++h) {
-            uint32_t pk[16];
-#pragma unroll
-            for (int c = 0; c < 16; ++c) {
-              const int e = h * 32 + 2 * c;
-              const uint64_t x = fma2(pair(s[e], s[e + 1]), scale2, off2);
-              uint64_t y;
-              float a, b;
-              if (C::kPolyEvery > 0 && (c % (C::kPolyEvery > 0 ? C::kPolyEvery : 1)) == 1) {
-                y = ex2_poly2(x);
-                unpair(y, a, b);
-                if (masked) {  // exactly zero
-                  a = e <= see ? a : 0.f;
-                  b = e + 1 <= see ? b : 0.f;
-                  y = pair(a, b);
+            const int r_end = it.kv_len - key0;  // V rows from here on are behind the item's keys
+            if (masked && (r_end < kRows || kAgain)) {
+              ok = bar_wait(&full[sv], (iv / NS) & 1, 521);
+              if (!ok) break;
+              uint8_t* v = smem + C::kRing + sv * C::kTileBytes;
+              constexpr int kChunks = D / 8;
+              for (int x = r_end * kChunks + t; x < kRows * kChunks; x += 128)
+                *reinterpret_cast<uint4*>(v + chunk_at<D>(x / kChunks, x % kChunks)) = make_uint4(0, 0, 0, 0);
+              fence_async_smem();
+              if constexpr (kAgain) {
+                const bool odd = odd_rows<D>(v, max(0, first_pos + 1 - key0), min(r_end, kRows), t);
+                // (any thread's finding is every thread's; once found it holds for the piece's later tiles too)
+                if (lane == 0) {
+                  if (odd) odd_v[w] = 1;
+                  mbar_arrive(&looked[w]);
                 }
-              } else {
+                ok = bar_wait(&looked[w], looks & 1, 523);
+                ++looks;
+                if (!ok) break;
+                by_hand = odd_v[w] != 0;
+              }
+            }
+          }
+          if (warp_on) {
+            float s[kRows];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) tmem_ld32(ts + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&s[c * 32]));
+            tc_wait_ld();
+            [[maybe_unused]] const float* sc =
+                reinterpret_cast<const float*>(smem + C::kScales) + ((tile0 + j) % C::kScaleRing) * 2 * kRows;
+            if constexpr (Q8) {
+#pragma unroll
+              for (int c = 0; c < kRows; c += 4) {
+                const float4 f = *reinterpret_cast<const float4*>(sc + c);
+                s[c] *= f.x, s[c + 1] *= f.y, s[c + 2] *= f.z, s[c + 3] *= f.w;
+              }
+            }
+            const int see = my_pos - key0;  // keys 0 .. see of the tile are this row's
+            if (masked) {
+#pragma unroll
+              for (int h = 0; h < kRows; h += 32) {
+                if (key0 + h + 31 > first_pos) {
+#pragma unroll
+                  for (int c = h; c < h + 32; ++c) s[c] = c <= see ? s[c] : -INFINITY;
+                }
+              }
+            }
+            float mx[4] = {m, m, m, m};
+#pragma unroll
+            for (int c = 0; c < kRows; c += 8) {
+#pragma unroll
+              for (int x = 0; x < 4; ++x) mx[x] = max3(mx[x], s[c + x], s[c + 4 + x]);
+            }
+            float m_new = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+            const bool grow = m == -INFINITY || (m_new - m) * p.scale_log2 > 8.f;
+            if (!grow) m_new = m;
+            if (i > 0 && __any_sync(0xffffffffu, grow)) {
+              const float f = m == -INFINITY ? 0.f : ex2((m - m_new) * p.scale_log2);
+              l2 = mul2(l2, pair(f, f));
+#pragma unroll 1
+              for (int c = 0; c < D; c += 32) {
+                uint32_t o[32];
+                tmem_ld32(to + c, o);
+                tc_wait_ld();
+#pragma unroll
+                for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
+                tmem_st32(to + c, o);
+              }
+            }
+            m = m_new;
+            const float off = m == -INFINITY ? 0.f : -m * p.scale_log2;
+            const uint64_t off2 = pair(off, off);
+            uint64_t sum[2] = {l2, 0};
+#pragma unroll
+            for (int h = 0; h < 4; ++h) {
+              uint32_t pk[16];
+#pragma unroll
+              for (int c = 0; c < 16; ++c) {
+                const int e = h * 32 + 2 * c;
+                const uint64_t x = fma2(pair(s[e], s[e + 1]), scale2, off2);
+                float a, b;
                 unpair(x, a, b);
                 a = ex2(a);
                 b = ex2(b);
-                y = pair(a, b);
-              }
-              sum[c & 1] = add2(sum[c & 1], y);
-              if constexpr (Q8) {  // the value's scale, with nothing of a masked key's
-                unpair(mul2(y, *reinterpret_cast<const uint64_t*>(sc + kRows + e)), a, b);
-                if (masked) {
-                  a = e <= see ? a : 0.f;
-                  b = e + 1 <= see ? b : 0.f;
-                }
-              }
-              pk[c] = pack_bf16x2(a, b);
-            }
-            tmem_st16(ts + h * 16, pk);
-          }
-          l2 = add2(sum[0], sum[1]);
-          tc_wait_st();
-          if constexpr (!Q8) {
-            if (by_hand) {
-              // O += P V over the keys that each row sees, from the stage, in the tensor cores' place
-              const uint8_t* v = smem + C::kRing + ((base + 2 * j + 1) % NS) * C::kTileBytes;
-#pragma unroll 1
-              for (int c = 0; c < D; c += 8) {
-                float o[8];
-                uint32_t u[8];
-                if (i > 0) {
-                  tmem_ld8(to + c, u);
-                  tc_wait_ld();
-                } else {
-#pragma unroll
-                  for (int x = 0; x < 8; ++x) u[x] = 0;
-                }
-#pragma unroll
-                for (int x = 0; x < 8; ++x) o[x] = __uint_as_float(u[x]);
-#pragma unroll 1
-                for (int q = 0; q < kRows; q += 16) {
-                  uint32_t pr[8];
-                  tmem_ld8(ts + q / 2, pr);
-                  tc_wait_ld();
-#pragma unroll
-                  for (int y = 0; y < 16; ++y) {
-                    const float pv = y & 1 ? bf16hi(pr[y / 2]) : bf16lo(pr[y / 2]);
-                    if (q + y <= see) {
-                      const uint4 x4 = *reinterpret_cast<const uint4*>(v + chunk_at<D>(q + y, c / 8));
-                      const uint32_t e[4] = {x4.x, x4.y, x4.z, x4.w};
-#pragma unroll
-                      for (int x = 0; x < 4; ++x) {
-                        o[2 * x] = fmaf(pv, bf16lo(e[x]), o[2 * x]);
-                        o[2 * x + 1] = fmaf(pv, bf16hi(e[x]), o[2 * x + 1]);
-                      }
-                    }
+                const uint64_t y = pair(a, b);
+                sum[c & 1] = add2(sum[c & 1], y);
+                if constexpr (Q8) {  // the value's scale, with nothing of a masked key's
+                  unpair(mul2(y, *reinterpret_cast<const uint64_t*>(sc + kRows + e)), a, b);
+                  if (masked) {
+                    a = e <= see ? a : 0.f;
+                    b = e + 1 <= see ? b : 0.f;
                   }
                 }
-#pragma unroll
-                for (int x = 0; x < 8; ++x) u[x] = __float_as_uint(o[x]);
-                tmem_st8(to + c, u);
+                pk[c] = pack_bf16x2(a, b);
               }
-              tc_wait_st();
+              tmem_st16(ts + h * 16, pk);
+            }
+            l2 = add2(sum[0], sum[1]);
+            tc_wait_st();
+            if constexpr (kAgain) {
+              if (by_hand) {
+                values_by_hand<D>(smem + C::kRing + ((base + 2 * j + 1) % NS) * C::kTileBytes, ts, to, see, i > 0);
+              }
             }
           }
+          if (kAgain && t == 0) skip[w] = by_hand;
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&pready[w]);
         }
-        if (!Q8 && t == 0) *(volatile int*)&skip[w] = by_hand;
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&pready[w]);
-      }
-      base += 2 * wk.tiles;
-      tile0 += wk.tiles;
-      if (!ok) break;
-      // ---------------- epilogue ----------------
-      float la, lb;
-      unpair(l2, la, lb);
-      float l = la + lb, ml = m == -INFINITY ? -INFINITY : m * p.scale_log2;
-      const bool both = wk.dual && wk.n1 > 0;  // two states of the same rows: the first warpgroup merges them
-      float2* mls = reinterpret_cast<float2*>(smem + C::kMl);
-      if (both && w == 1) {
-        mls[t] = make_float2(ml, l);
-        ok = bar_wait(&ofull[1], co++ & 1, 522);
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(mlready);
-        ok = ok && bar_wait(merged, duals++ & 1, 528);
+        base += 2 * wk.tiles;
+        tile0 += wk.tiles;
+        if (!ok) break;
+        // ---------------- epilogue ----------------
+        float la, lb;
+        unpair(l2, la, lb);
+        float l = la + lb, ml = m == -INFINITY ? -INFINITY : m * p.scale_log2;
+        const bool both = wk.dual && wk.n1 > 0;  // two states of the same rows: the first warpgroup merges them
+        float2* mls = reinterpret_cast<float2*>(smem + C::kMl);
+        if (both && w == 1) {
+          mls[t] = make_float2(ml, l);
+          ok = bar_wait(&ofull[1], co++ & 1, 522);
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(mlready);
+          ok = ok && bar_wait(merged, duals++ & 1, 528);
+          if (!ok) break;
+          tc_fence_after();
+          continue;
+        }
+        if (n == 0) {  // a part of a split item whose keys lie behind all of the first row tile's: an empty state
+          if (it.slot >= 0 && t < valid)
+            p.ws_ml[((int64_t)it.slot * p.hkv + wk.head) * (2 * kRows) + w * kRows + t] = make_float2(-INFINITY, 0.f);
+          continue;
+        }
+        ok = bar_wait(&ofull[w], co++ & 1, 522);
+        float f0 = 1.f, f1 = 0.f;
+        if (both) {
+          ok = ok && bar_wait(mlready, duals++ & 1, 529);
+          const float2 o1 = mls[t];
+          const float top = fmaxf(ml, o1.x);
+          f0 = ml == -INFINITY ? 0.f : exp2f(ml - top);
+          f1 = o1.x == -INFINITY ? 0.f : exp2f(o1.x - top);
+          l = (f0 == 0.f ? 0.f : f0 * l) + (f1 == 0.f ? 0.f : f1 * o1.y);
+          ml = top;
+        }
         if (!ok) break;
         tc_fence_after();
-        continue;
-      }
-      if (n == 0) {  // a part of a split item whose keys lie behind all of the first row tile's: an empty state
-        if (it.slot >= 0 && t < valid)
-          p.ws_ml[((int64_t)it.slot * p.hkv + wk.head) * (2 * kRows) + w * kRows + t] = make_float2(-INFINITY, 0.f);
-        continue;
-      }
-      ok = bar_wait(&ofull[w], co++ & 1, 522);
-      float f0 = 1.f, f1 = 0.f;
-      if (both) {
-        ok = ok && bar_wait(mlready, duals++ & 1, 529);
-        const float2 o1 = mls[t];
-        const float top = fmaxf(ml, o1.x);
-        f0 = ml == -INFINITY ? 0.f : exp2f(ml - top);
-        f1 = o1.x == -INFINITY ? 0.f : exp2f(o1.x - top);
-        l = (f0 == 0.f ? 0.f : f0 * l) + (f1 == 0.f ? 0.f : f1 * o1.y);
-        ml = top;
-      }
-      if (!ok) break;
-      tc_fence_after();
-      if (warp_on) {
-        const float inv = it.slot >= 0 ? 1.f : (l == 0.f ? 0.f : 1.f / l);
-        f0 *= inv;
-        f1 *= inv;
-        const int64_t slot_row = ((int64_t)it.slot * p.hkv + wk.head) * (2 * kRows) + (wk.dual ? 0 : w * kRows) + t;
-        __nv_bfloat16* dst = p.out + (int64_t)(it.row0 + tok0) * row_stride + (int64_t)wk.head * p.group * D + my_off;
+        if (warp_on) {
+          float odd_sum = 0.f;  // a NaN once a value is one, or an infinity
+          const float inv = it.slot >= 0 ? 1.f : (l == 0.f ? 0.f : 1.f / l);
+          f0 *= inv;
+          f1 *= inv;
+          const int64_t slot_row = ((int64_t)it.slot * p.hkv + wk.head) * (2 * kRows) + (wk.dual ? 0 : w * kRows) + t;
+          __nv_bfloat16* dst = p.out + (int64_t)(it.row0 + tok0) * row_stride + (int64_t)wk.head * p.group * D + my_off;
 #pragma unroll 1
-        for (int c = 0; c < D; c += 32) {
-          uint32_t o[32];
-          tmem_ld32(to + c, o);
-          tc_wait_ld();
-#pragma unroll
-          for (int x = 0; x < 32; ++x) o[x] = f0 == 0.f ? 0u : __float_as_uint(__uint_as_float(o[x]) * f0);
-          if (both) {
-            uint32_t o1[32];
-            tmem_ld32(to + D + c, o1);
+          for (int c = 0; c < D; c += 32) {
+            uint32_t o[32];
+            tmem_ld32(to + c, o);
             tc_wait_ld();
 #pragma unroll
-            for (int x = 0; x < 32; ++x)
-              if (f1 != 0.f) o[x] = __float_as_uint(fmaf(__uint_as_float(o1[x]), f1, __uint_as_float(o[x])));
-          }
-          if (t < valid) {
-            if (it.slot < 0) {
+            for (int x = 0; x < 32; ++x) o[x] = f0 == 0.f ? 0u : __float_as_uint(__uint_as_float(o[x]) * f0);
+            if (both) {
+              uint32_t o1[32];
+              tmem_ld32(to + D + c, o1);
+              tc_wait_ld();
 #pragma unroll
-              for (int x = 0; x < 32; x += 8)
-                *reinterpret_cast<uint4*>(dst + c + x) =
-                    make_uint4(pack_bf16x2(__uint_as_float(o[x]), __uint_as_float(o[x + 1])),
-                               pack_bf16x2(__uint_as_float(o[x + 2]), __uint_as_float(o[x + 3])),
-                               pack_bf16x2(__uint_as_float(o[x + 4]), __uint_as_float(o[x + 5])),
-                               pack_bf16x2(__uint_as_float(o[x + 6]), __uint_as_float(o[x + 7])));
-            } else {
+              for (int x = 0; x < 32; ++x)
+                if (f1 != 0.f) o[x] = __float_as_uint(fmaf(__uint_as_float(o1[x]), f1, __uint_as_float(o[x])));
+            }
+            if constexpr (!Q8) {
 #pragma unroll
-              for (int x = 0; x < 32; x += 4)
-                *reinterpret_cast<uint4*>(p.ws_o + slot_row * D + c + x) = make_uint4(o[x], o[x + 1], o[x + 2], o[x + 3]);
+              for (int x = 0; x < 32; ++x) odd_sum = fmaf(__uint_as_float(o[x]), 0.f, odd_sum);
+            }
+            if (t < valid) {
+              if (it.slot < 0) {
+#pragma unroll
+                for (int x = 0; x < 32; x += 8)
+                  *reinterpret_cast<uint4*>(dst + c + x) =
+                      make_uint4(pack_bf16x2(__uint_as_float(o[x]), __uint_as_float(o[x + 1])),
+                                 pack_bf16x2(__uint_as_float(o[x + 2]), __uint_as_float(o[x + 3])),
+                                 pack_bf16x2(__uint_as_float(o[x + 4]), __uint_as_float(o[x + 5])),
+                                 pack_bf16x2(__uint_as_float(o[x + 6]), __uint_as_float(o[x + 7])));
+              } else {
+#pragma unroll
+                for (int x = 0; x < 32; x += 4)
+                  *reinterpret_cast<uint4*>(p.ws_o + slot_row * D + c + x) = make_uint4(o[x], o[x + 1], o[x + 2], o[x + 3]);
+              }
             }
           }
+          if (it.slot >= 0 && t < valid) p.ws_ml[slot_row] = make_float2(ml, l);
+          if (!Q8 && !kAgain && t < valid && odd_sum != 0.f) {
+            // Zero times an infinite or NaN value of a masked key may be in there: the piece is done over with a look at V.
+            atomicOr(const_cast<uint32_t*>(redo + min(piece >> 5, kRedoWords - 1)), 1u << (piece < 32 * kRedoWords ? piece & 31 : 31));
+            *redo_any = 1;
+          }
         }
-        if (it.slot >= 0 && t < valid) p.ws_ml[slot_row] = make_float2(ml, l);
+        tc_fence_before();
+        if (both) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(merged);
+        }
       }
-      tc_fence_before();
-      if (both) {
-        __syncwarp();
-        if (lane == 0) mbar_arrive(merged);
-      }
+    };
+    softmax_pass(std::false_type{});
+    if constexpr (!Q8) {
+      block_barrier();
+      if (*redo_any) softmax_pass(std::true_type{});
     }
   }
   tc_fence_before();

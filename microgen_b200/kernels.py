@@ -7,6 +7,7 @@ current CUDA stream. Tensors must live on a CUDA device; there is no CPU path.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 
 import torch
 
@@ -249,18 +250,47 @@ class RaggedPlan:
         self.work = torch.zeros(n.value, dtype=torch.uint8, device=self.device)
         self.workspace = torch.empty(ws.value, dtype=torch.uint8, device=self.device)
         self.tables: torch.Tensor | None = None
+        # the arguments of ragged_plan and ragged_attn that stay with the plan
+        self.out_args = (self.hq, self.hkv, self.d, *(t.data_ptr() for t in (
+            self.cu_rows, self.kv_lens, self.positions, self.slots, self.seq_ids, self.n_blocks, self.cursor, self.work)),
+            self.work.numel())
+        self.workspace_args = (self.workspace.data_ptr(), self.workspace.numel())
 
 
-def _on(device, **tensors) -> None:
-    for name, t in tensors.items():
-        if t is not None and t.device != device:
-            raise ValueError(f"{name} is on {t.device}, expected {device}")
+# The checks and the call cost a serving step host time at every layer, so they are kept to a few hundred nanoseconds
+# a tensor: one test of everything, and the words for what is wrong only where something is.
+def _wrong(t, name: str, dtype, dev: int, shape) -> None:
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor (the ragged path has no CPU fallback)")
+    if t.dtype is not dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.get_device() != dev:
+        raise ValueError(f"{name} is on {t.device}, expected cuda:{dev}")
+    if shape is not None and t.shape != shape:
+        raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
+    raise ValueError(f"{name} must be contiguous")
 
 
-def _vec_i32(t, n, name: str) -> None:
-    _need(t, torch.int32, name)
-    if t.dim() != 1 or (n is not None and t.shape[0] != n):
-        raise ValueError(f"{name} must be int32 [{n if n is not None else 'n'}], got {tuple(t.shape)}")
+def _check(t, name: str, dtype, dev: int, shape=None) -> None:
+    if t.dtype is not dtype or t.get_device() != dev or (shape is not None and t.shape != shape) or not t.is_contiguous():
+        _wrong(t, name, dtype, dev, shape)
+
+
+def _addr(t) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+
+
+def _call_on(dev: int, name: str, *args) -> None:
+    """``_lib.call`` on device ``dev``'s current stream (appended to ``args``), with that device current."""
+    if torch.cuda.current_device() == dev:
+        _lib.call(name, *args, _raw_stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            _lib.call(name, *args, _raw_stream(dev))
 
 
 def ragged_plan(plan: RaggedPlan, q_lens, ctx_lens, tables, num_blocks: int, n_blocks=None, free_blocks=None,
@@ -273,53 +303,44 @@ def ragged_plan(plan: RaggedPlan, q_lens, ctx_lens, tables, num_blocks: int, n_b
     ``tables``. ``plan.n_blocks`` and ``plan.cursor`` hold the counts after the step and may be passed back in (as
     may ``plan.kv_lens`` for ctx_lens). Impossible lengths or an exhausted list make an empty plan, and
     ``check_device`` raises."""
-    _vec_i32(q_lens, plan.b, "q_lens")
-    _vec_i32(ctx_lens, plan.b, "ctx_lens")
-    _need(tables, torch.int32, "tables")
-    if tables.shape != (plan.b, plan.max_blocks):
-        raise ValueError(f"tables must be [{plan.b}, {plan.max_blocks}], got {tuple(tables.shape)}")
+    dev, i32, b = plan.device.index, torch.int32, plan.b
+    _check(q_lens, "q_lens", i32, dev, (b,))
+    _check(ctx_lens, "ctx_lens", i32, dev, (b,))
+    _check(tables, "tables", i32, dev, (b, plan.max_blocks))
     if n_blocks is not None:
-        _vec_i32(n_blocks, plan.b, "n_blocks")
+        _check(n_blocks, "n_blocks", i32, dev, (b,))
+    n_free = 0
     if free_blocks is not None:
-        _vec_i32(free_blocks, None, "free_blocks")
+        n_free = free_blocks.numel()
+        _check(free_blocks, "free_blocks", i32, dev, (n_free,))
     if cursor is not None:
         if free_blocks is None:
             raise ValueError("a cursor needs the free list it counts in")
-        _vec_i32(cursor, 1, "cursor")
-    _on(plan.device, q_lens=q_lens, ctx_lens=ctx_lens, tables=tables, n_blocks=n_blocks, free_blocks=free_blocks,
-        cursor=cursor)
-    # an empty free list still has an address, so that running out of it is noticed
-    free = free_blocks if free_blocks is None or free_blocks.numel() else plan.cursor
-    with torch.cuda.device(plan.device):
-        _lib.call("mg_ragged_plan", _ptr(q_lens), _ptr(ctx_lens), plan.b, plan.max_rows, _ptr(tables), plan.max_blocks,
-                  int(num_blocks), _ptr(n_blocks), _ptr(free), 0 if free_blocks is None else free_blocks.numel(),
-                  _ptr(cursor), plan.hq, plan.hkv, plan.d, _ptr(plan.cu_rows), _ptr(plan.kv_lens),
-                  _ptr(plan.positions), _ptr(plan.slots), _ptr(plan.seq_ids), _ptr(plan.n_blocks), _ptr(plan.cursor),
-                  _ptr(plan.work), plan.work.numel(), _stream())
+        _check(cursor, "cursor", i32, dev, (1,))
+    # an empty free list has no address: any stands for it, so that running out of it is noticed
+    free = 0 if free_blocks is None else (free_blocks.data_ptr() or plan.cursor.data_ptr())
+    _call_on(dev, "mg_ragged_plan", q_lens.data_ptr(), ctx_lens.data_ptr(), b, plan.max_rows, tables.data_ptr(),
+             plan.max_blocks, int(num_blocks), _addr(n_blocks), free, n_free, _addr(cursor), *plan.out_args)
     plan.tables = tables
     return plan
 
 
-def _pools(k_pool, v_pool, k_scales, v_scales, hkv: int, d: int) -> bool:
-    """Check a K/V pool pair (and its scales when int8); True for int8."""
-    q8 = k_pool.dtype == torch.int8
+def _pools(k_pool, v_pool, k_scales, v_scales, hkv: int, d: int, dev: int) -> None:
+    """Check a K/V pool pair, and its scales when int8."""
+    q8 = k_pool.dtype is torch.int8
+    want = (k_pool.shape[0] if k_pool.dim() else 0, hkv, BLOCK_SIZE, d)
     dt = torch.int8 if q8 else torch.bfloat16
-    _need(k_pool, dt, "k_pool")
-    _need(v_pool, dt, "v_pool")
-    want = (k_pool.shape[0], hkv, BLOCK_SIZE, d)
-    if tuple(k_pool.shape) != want or tuple(v_pool.shape) != want or want[0] < 1:
-        raise ValueError(f"pools must be [num_blocks, {hkv}, {BLOCK_SIZE}, {d}], got {tuple(k_pool.shape)} and "
-                         f"{tuple(v_pool.shape)}")
-    if not q8 and (k_scales is not None or v_scales is not None):
-        raise ValueError("scales belong to int8 pools")
+    _check(k_pool, "k_pool", dt, dev, want)
+    _check(v_pool, "v_pool", dt, dev, want)
+    if want[0] < 1:
+        raise ValueError("the pools hold no block")
     if q8:
-        for t, name in ((k_scales, "k_scales"), (v_scales, "v_scales")):
-            if t is None:
-                raise ValueError(f"int8 pools need {name}")
-            _need(t, torch.float32, name)
-            if tuple(t.shape) != want[:3]:
-                raise ValueError(f"{name} must be {list(want[:3])}, got {tuple(t.shape)}")
-    return q8
+        if k_scales is None or v_scales is None:
+            raise ValueError("int8 pools need k_scales and v_scales")
+        _check(k_scales, "k_scales", torch.float32, dev, want[:3])
+        _check(v_scales, "v_scales", torch.float32, dev, want[:3])
+    elif k_scales is not None or v_scales is not None:
+        raise ValueError("scales belong to int8 pools")
 
 
 def norm_rope_kv_append(qkv, positions, cos_sin, slots, hq, hkv, d, k_pool, v_pool, q_weight=None, k_weight=None,
@@ -330,39 +351,35 @@ def norm_rope_kv_append(qkv, positions, cos_sin, slots, hq, hkv, d, k_pool, v_po
     whose slot is negative are padding and left alone: with padding rows pass ``q_out``, whose rows then stay."""
     if not qkv.is_cuda or qkv.dtype not in (torch.float32, torch.bfloat16):
         raise TypeError("qkv must be a CUDA tensor, fp32 or bf16 (the ragged path has no CPU fallback)")
-    rows = qkv.shape[0]
-    if qkv.dim() != 2 or qkv.shape[1] != (hq + 2 * hkv) * d or qkv.stride(1) != 1:
-        raise ValueError(f"qkv must be [rows, {(hq + 2 * hkv) * d}] with unit inner stride, got {tuple(qkv.shape)}")
-    ld = qkv.stride(0) if rows > 1 else qkv.shape[1]
-    if ld < qkv.shape[1] or ld % 4:
+    width = (hq + 2 * hkv) * d
+    if qkv.dim() != 2 or qkv.shape[1] != width or qkv.stride(1) != 1:
+        raise ValueError(f"qkv must be [rows, {width}] with unit inner stride, got {list(qkv.shape)}")
+    rows, dev = qkv.shape[0], qkv.get_device()
+    ld = qkv.stride(0) if rows > 1 else width
+    if ld < width or ld % 4:
         raise ValueError("rows of qkv must not overlap, and start a multiple of 4 elements apart")
-    _vec_i32(slots, rows, "slots")
+    _check(slots, "slots", torch.int32, dev, (rows,))
+    max_pos = pos = 0
     if cos_sin is not None:
-        _need(cos_sin, torch.float32, "cos_sin")
-        if cos_sin.dim() != 2 or cos_sin.shape[1] != d:
-            raise ValueError(f"cos_sin must be [max_pos, {d}]")
-        _vec_i32(positions, rows, "positions")
-    for t, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
-        if t is not None:
-            _need(t, torch.float32, name)
-            if tuple(t.shape) != (d,):
-                raise ValueError(f"{name} must be [{d}]")
-    _pools(k_pool, v_pool, k_scales, v_scales, hkv, d)
+        max_pos = cos_sin.shape[0]
+        _check(cos_sin, "cos_sin", torch.float32, dev, (max_pos, d))
+        _check(positions, "positions", torch.int32, dev, (rows,))
+        pos = positions.data_ptr()
+    if q_weight is not None:
+        _check(q_weight, "q_weight", torch.float32, dev, (d,))
+    if k_weight is not None:
+        _check(k_weight, "k_weight", torch.float32, dev, (d,))
+    _pools(k_pool, v_pool, k_scales, v_scales, hkv, d, dev)
     if q_out is None:
         q_out = torch.empty((rows, hq, d), dtype=torch.bfloat16, device=qkv.device)
-    if q_out.dtype not in (torch.float32, torch.bfloat16):
-        raise TypeError("q_out must be bf16 or fp32")
-    _need(q_out, q_out.dtype, "q_out")
-    if q_out.numel() != rows * hq * d:
-        raise ValueError(f"q_out must be [{rows}, {hq}, {d}]")
-    _on(qkv.device, positions=positions if cos_sin is not None else None, cos_sin=cos_sin, slots=slots, k_pool=k_pool,
-        v_pool=v_pool, q_weight=q_weight, k_weight=k_weight, q_out=q_out, k_scales=k_scales, v_scales=v_scales)
-    with torch.cuda.device(qkv.device):
-        _lib.call("mg_norm_rope_kv_append", _ptr(qkv), int(qkv.dtype == torch.bfloat16), ld, rows,
-                  _ptr(positions if cos_sin is not None else None), _ptr(cos_sin),
-                  0 if cos_sin is None else cos_sin.shape[0], _ptr(slots), _ptr(q_weight), _ptr(k_weight), float(eps),
-                  hq, hkv, d, _ptr(q_out), int(q_out.dtype == torch.bfloat16), _ptr(k_pool), _ptr(v_pool),
-                  _ptr(k_scales), _ptr(v_scales), k_pool.shape[0], _stream())
+    else:
+        if q_out.dtype not in (torch.float32, torch.bfloat16):
+            raise TypeError("q_out must be bf16 or fp32")
+        _check(q_out, "q_out", q_out.dtype, dev, (rows, hq, d))
+    _call_on(dev, "mg_norm_rope_kv_append", qkv.data_ptr(), int(qkv.dtype is torch.bfloat16), ld, rows, pos,
+             _addr(cos_sin), max_pos, slots.data_ptr(), _addr(q_weight), _addr(k_weight), eps, hq, hkv, d,
+             q_out.data_ptr(), int(q_out.dtype is torch.bfloat16), k_pool.data_ptr(), v_pool.data_ptr(),
+             _addr(k_scales), _addr(v_scales), k_pool.shape[0])
     return q_out
 
 
@@ -372,29 +389,25 @@ def ragged_attn(q, k_pool, v_pool, plan: RaggedPlan, scale, out=None, k_scales=N
     scales. Returns bf16 [rows, hq*d]. The step's own K/V must already be in the pools."""
     if plan.tables is None:
         raise ValueError("the plan has not been filled: call ragged_plan first")
-    _need(q, torch.bfloat16, "q")
-    if q.dim() != 3 or tuple(q.shape[1:]) != (plan.hq, plan.d):
-        raise ValueError(f"q must be [rows, {plan.hq}, {plan.d}], got {tuple(q.shape)}")
-    _pools(k_pool, v_pool, k_scales, v_scales, plan.hkv, plan.d)
-    if not float(scale) > 0.0:
+    dev, hq, d = plan.device.index, plan.hq, plan.d
+    rows = q.shape[0] if q.dim() else 0
+    _check(q, "q", torch.bfloat16, dev, (rows, hq, d))
+    _pools(k_pool, v_pool, k_scales, v_scales, plan.hkv, d, dev)
+    if not scale > 0.0:
         raise ValueError("scale must be positive")
-    rows = q.shape[0]
     if out is None:
-        out = torch.empty((rows, plan.hq * plan.d), dtype=torch.bfloat16, device=q.device)
-    _need(out, torch.bfloat16, "out")
-    if out.numel() != rows * plan.hq * plan.d:
-        raise ValueError(f"out must be [{rows}, {plan.hq * plan.d}]")
-    _on(plan.device, q=q, k_pool=k_pool, v_pool=v_pool, out=out, k_scales=k_scales, v_scales=v_scales)
-    with torch.cuda.device(plan.device):
-        _lib.call("mg_ragged_attn", _ptr(q), rows, _ptr(k_pool), _ptr(v_pool), _ptr(k_scales), _ptr(v_scales),
-                  k_pool.shape[0], _ptr(plan.tables), plan.max_blocks, plan.b, plan.max_rows, plan.hq, plan.hkv,
-                  plan.d, float(scale), _ptr(plan.work), _ptr(out), _ptr(plan.workspace), plan.workspace.numel(),
-                  _stream())
+        out = torch.empty((rows, hq * d), dtype=torch.bfloat16, device=q.device)
+    else:
+        _check(out, "out", torch.bfloat16, dev, (rows, hq * d))
+    _call_on(dev, "mg_ragged_attn", q.data_ptr(), rows, k_pool.data_ptr(), v_pool.data_ptr(), _addr(k_scales),
+             _addr(v_scales), k_pool.shape[0], plan.tables.data_ptr(), plan.max_blocks, plan.b, plan.max_rows, hq,
+             plan.hkv, d, scale, plan.work.data_ptr(), out.data_ptr(), *plan.workspace_args)
     if rows:
         _lib.LAUNCHES[0] += 1  # the merge of split items
     return out
 
 
+@functools.lru_cache(maxsize=256)
 def verify_workspace_bytes(rows: int, vocab: int) -> int:
     n = C.c_size_t(0)
     _lib.call("mg_verify_workspace_bytes", int(rows), int(vocab), C.byref(n))
@@ -410,47 +423,44 @@ def verify_drafts(logits, tokens, cu_rows, uniforms, draft_probs=None, temperatu
     (so row r asks about tokens[r+1]); ``uniforms`` fp32 [rows] in [0, 1); ``draft_probs`` fp32 [rows, vocab], the
     draft's distribution at each asking row (None: the drafts were certain); ``temperatures`` fp32 [b] (None: 1; 0:
     greedy). Returns (accepted int32 [b], next token int32 [b]); see ``mg_verify_drafts`` for the rule."""
-    _need(logits, torch.float32, "logits", contiguous=False)
     if logits.dim() != 2 or logits.stride(1) != 1 or logits.shape[1] < 1:
         raise ValueError("logits must be [rows, vocab] with unit inner stride")
     rows, vocab = logits.shape
+    dev, f32, i32 = logits.get_device(), torch.float32, torch.int32
+    if dev < 0 or logits.dtype is not f32:
+        _wrong(logits, "logits", f32, dev, None)
     ld = logits.stride(0) if rows > 1 else vocab
-    _vec_i32(tokens, rows, "tokens")
-    _vec_i32(cu_rows, None, "cu_rows")
-    b = cu_rows.shape[0] - 1
+    _check(tokens, "tokens", i32, dev, (rows,))
+    b = cu_rows.numel() - 1
     if b < 0:
         raise ValueError("cu_rows must be int32 [b + 1]")
-    _need(uniforms, torch.float32, "uniforms")
-    if tuple(uniforms.shape) != (rows,):
-        raise ValueError(f"uniforms must be [{rows}]")
+    _check(cu_rows, "cu_rows", i32, dev, (b + 1,))
+    _check(uniforms, "uniforms", f32, dev, (rows,))
     ldq = vocab
     if draft_probs is not None:
-        _need(draft_probs, torch.float32, "draft_probs", contiguous=False)
-        if tuple(draft_probs.shape) != (rows, vocab) or draft_probs.stride(1) != 1:
+        if draft_probs.shape != (rows, vocab) or draft_probs.stride(1) != 1:
             raise ValueError(f"draft_probs must be [{rows}, {vocab}] with unit inner stride")
+        if draft_probs.dtype is not f32 or draft_probs.get_device() != dev:
+            _wrong(draft_probs, "draft_probs", f32, dev, None)
         ldq = draft_probs.stride(0) if rows > 1 else vocab
     if ld < vocab or ldq < vocab:
         raise ValueError("rows of logits and draft_probs must not overlap")
     if temperatures is not None:
-        _need(temperatures, torch.float32, "temperatures")
-        if tuple(temperatures.shape) != (b,):
-            raise ValueError(f"temperatures must be [{b}]")
-    dev = logits.device
-    if accepted is None:
-        accepted = torch.empty(b, dtype=torch.int32, device=dev)
-    if next_tokens is None:
-        next_tokens = torch.empty(b, dtype=torch.int32, device=dev)
-    _vec_i32(accepted, b, "accepted")
-    _vec_i32(next_tokens, b, "next_tokens")
-    with torch.cuda.device(dev):
-        ws = verify_workspace_bytes(rows, vocab)
-        if workspace is None or workspace.numel() * workspace.element_size() < ws:
-            workspace = torch.empty(ws, dtype=torch.uint8, device=dev)
-        _on(dev, tokens=tokens, cu_rows=cu_rows, uniforms=uniforms, draft_probs=draft_probs, temperatures=temperatures,
-            accepted=accepted, next_tokens=next_tokens, workspace=workspace)
-        _lib.call("mg_verify_drafts", _ptr(logits), ld, rows, vocab, _ptr(tokens), _ptr(cu_rows), b, _ptr(draft_probs),
-                  ldq, _ptr(uniforms), _ptr(temperatures), _ptr(accepted), _ptr(next_tokens), _ptr(workspace), ws,
-                  _stream())
+        _check(temperatures, "temperatures", f32, dev, (b,))
+    if accepted is None or next_tokens is None:
+        both = torch.empty((2, b), dtype=i32, device=logits.device)
+        accepted = both[0] if accepted is None else accepted
+        next_tokens = both[1] if next_tokens is None else next_tokens
+    _check(accepted, "accepted", i32, dev, (b,))
+    _check(next_tokens, "next_tokens", i32, dev, (b,))
+    ws = verify_workspace_bytes(rows, vocab)
+    if workspace is None or workspace.numel() * workspace.element_size() < ws:
+        workspace = torch.empty(ws, dtype=torch.uint8, device=logits.device)
+    elif workspace.get_device() != dev or not workspace.is_contiguous():
+        raise ValueError("workspace must be contiguous, and on the device of logits")
+    _call_on(dev, "mg_verify_drafts", logits.data_ptr(), ld, rows, vocab, tokens.data_ptr(), cu_rows.data_ptr(), b,
+             _addr(draft_probs), ldq, uniforms.data_ptr(), _addr(temperatures), accepted.data_ptr(),
+             next_tokens.data_ptr(), workspace.data_ptr(), ws)
     if rows and b:
         _lib.LAUNCHES[0] += 1  # the row statistics, then the decision
     return accepted, next_tokens

@@ -926,18 +926,39 @@ __global__ void __launch_bounds__(kMergeWarps * 32) ragged_merge_kernel(const Ra
     const int tok = r / p.group, w = tok / p.tok_tile;
     const int at = w * kRows + r - w * p.tok_tile * p.group;
     const int64_t first = ((int64_t)g.slot0 * p.hkv + kvh) * (2 * kRows) + at, step = (int64_t)p.hkv * (2 * kRows);
+    // every lane holds the state of every 32nd part; the parts' outputs are read eight at a time
     float M = -INFINITY;
     for (int s = lane; s < g.parts; s += 32) M = fmaxf(M, p.ws_ml[first + s * step].x);
     M = warp_max(M);
     float L = 0.f, o[D / 32] = {};
-    for (int s = 0; s < g.parts; ++s) {
-      const float2 ml = p.ws_ml[first + s * step];
-      const float f = ml.x == -INFINITY ? 0.f : exp2f(ml.x - M);
-      L += f * ml.y;
-      const float* src = p.ws_o + (first + s * step) * D + lane * (D / 32);
+    for (int s0 = 0; s0 < g.parts; s0 += 32) {
+      float f = 0.f;
+      if (s0 + lane < g.parts) {
+        const float2 ml = p.ws_ml[first + (s0 + lane) * step];
+        f = ml.x == -INFINITY ? 0.f : exp2f(ml.x - M);
+        L += f == 0.f ? 0.f : f * ml.y;
+      }
+      const int n = min(32, g.parts - s0);
+#pragma unroll 1
+      for (int s = 0; s < n; s += 8) {
+        float v[8][D / 32];
 #pragma unroll
-      for (int x = 0; x < D / 32; ++x) o[x] += f == 0.f ? 0.f : f * src[x];
+        for (int y = 0; y < 8; ++y) {
+          const float* src = p.ws_o + (first + (s0 + min(s + y, n - 1)) * step) * D + lane * (D / 32);
+#pragma unroll
+          for (int x = 0; x < D / 32; ++x) v[y][x] = src[x];
+        }
+#pragma unroll
+        for (int y = 0; y < 8; ++y) {
+          const float fy = __shfl_sync(0xffffffffu, f, (s + y) & 31);
+          if (s + y < n && fy != 0.f) {
+#pragma unroll
+            for (int x = 0; x < D / 32; ++x) o[x] = fmaf(fy, v[y][x], o[x]);
+          }
+        }
+      }
     }
+    L = warp_sum(L);
     const float inv = L == 0.f ? 0.f : 1.f / L;
     __nv_bfloat16* dst = p.out + (int64_t)(g.row0 + tok) * p.hq * D + ((int64_t)kvh * p.group + r % p.group) * D + lane * (D / 32);
 #pragma unroll

@@ -23,6 +23,8 @@ constexpr int kStatChunk = kStatThreads * 4 * kStatVec;  // logits per CTA
 constexpr int kPickThreads = 512;
 constexpr int kPickWarps = kPickThreads / 32;
 constexpr int kPickCtas = 8;
+constexpr int kPickBatch = 8;                            // loads in flight per thread
+constexpr int kPickStore = 200 * 1024;                   // shared memory for a CTA's share of the weights
 
 struct VerifyArgs {
   const float* logits;
@@ -51,14 +53,6 @@ __global__ void __launch_bounds__(kStatThreads) verify_stats_kernel(const Verify
   __shared__ int32_t sm_i[kStatThreads / 32];
   const int64_t row = blockIdx.y;
   const int t = threadIdx.x, lane = t & 31, w = t >> 5;
-  // the request that owns the row: the starts at or before it, less one
-  int seen = 0;
-  for (int i0 = 0; i0 <= p.b; i0 += kStatThreads)
-    seen += __syncthreads_count(i0 + t <= p.b && p.cu[i0 + t] <= row);
-  const int req = seen - 1;
-  if (req < 0 || req >= p.b) return;  // a row behind the last request
-  const float T = p.temps ? p.temps[req] : 1.f;
-  const float c = T > 0.f ? 1.4426950408889634f / T : 0.f;
   const float* x = p.logits + row * p.ld;
   const int64_t lo = (int64_t)blockIdx.x * kStatChunk, hi = min(lo + (int64_t)kStatChunk, p.vocab);
   float v[4 * kStatVec];
@@ -74,6 +68,14 @@ __global__ void __launch_bounds__(kStatThreads) verify_stats_kernel(const Verify
       for (int e = 0; e < 4; ++e) v[4 * k + e] = i + e < hi ? x[i + e] : -INFINITY;
     }
   }
+  // (while the loads are under way) the request that owns the row: the starts at or before it, less one
+  int seen = 0;
+  for (int i0 = 0; i0 <= p.b; i0 += kStatThreads)
+    seen += __syncthreads_count(i0 + t <= p.b && p.cu[i0 + t] <= row);
+  const int req = seen - 1;
+  if (req < 0 || req >= p.b) return;  // a row behind the last request
+  const float T = p.temps ? p.temps[req] : 1.f;
+  const float c = T > 0.f ? 1.4426950408889634f / T : 0.f;
   float m = -INFINITY, s = 0.f, best = -INFINITY;
   int32_t bi = 0x7fffffff;
   if (T > 0.f) {
@@ -192,7 +194,9 @@ __device__ __forceinline__ double cluster_total(double mine, double* part, int w
   return warp_sum_d(total);
 }
 
+template <bool kStored>
 __global__ void __launch_bounds__(kPickThreads) verify_pick_kernel(const VerifyArgs p) {
+  extern __shared__ double weights[];
   griddep_launch();
   griddep_wait();
   __shared__ int s_stop, s_bad;
@@ -271,67 +275,103 @@ __global__ void __launch_bounds__(kPickThreads) verify_pick_kernel(const VerifyA
   const float* qrow = stop < n && p.probs ? p.probs + (r0 + stop) * p.ldq : nullptr;
   const int64_t hole = stop < n && !p.probs ? (int64_t)p.tokens[r0 + stop + 1] : -1;  // a one-hot draft's token
   const double mx = (double)s_max, inv_t = 1.0 / (double)T;
-  // each warp owns a contiguous run of the vocabulary, in groups of 32
-  const int64_t groups = (p.vocab + 31) / 32, nw = kPickCtas * kPickWarps;
+  // each warp owns a contiguous run of the vocabulary; in the stored form its weights stay in shared memory
+  const int64_t nw = kPickCtas * kPickWarps, run = (p.vocab + nw - 1) / nw;
   const int64_t me = (int64_t)rank * kPickWarps + w;
-  const int64_t g0 = me * groups / nw, g1 = (me + 1) * groups / nw;
-  auto weight = [&](int64_t v) -> double { return v < p.vocab ? exp(((double)x[v] - mx) * inv_t) : 0.0; };
+  const int64_t v0 = min(me * run, p.vocab);
+  const int len = (int)(min(v0 + run, p.vocab) - v0);
+  double* kept = weights + (kStored ? (int64_t)w * run : 0);
+  auto weight = [&](int64_t v) -> double { return exp(((double)x[v] - mx) * inv_t); };
   double z = 0.0, holed = 0.0;
-  for (int64_t g = g0; g < g1; ++g) {
-    const int64_t v = g * 32 + lane;
-    const double e = weight(v);
-    z += e;
-    if (v != hole) holed += e;
+  for (int i0 = lane; i0 < len; i0 += 32 * kPickBatch) {
+    float l[kPickBatch];
+#pragma unroll
+    for (int k = 0; k < kPickBatch; ++k) l[k] = i0 + 32 * k < len ? __ldg(x + v0 + i0 + 32 * k) : 0.f;
+#pragma unroll
+    for (int k = 0; k < kPickBatch; ++k) {
+      const int i = i0 + 32 * k;
+      if (i < len) {
+        double e = exp(((double)l[k] - mx) * inv_t);
+        z += e;
+        if (v0 + i == hole) e = 0.0;  // nothing is left of it
+        holed += e;
+        if (kStored) kept[i] = e;
+      }
+    }
   }
   z = warp_sum_d(z);
-  const double Z = cluster_total(z, part_z, w, lane, nullptr);
-  // r(v): the rest that is drawn from, scaled so that it needs no second normalisation
-  bool plain = stop >= n;  // nothing to take away
-  auto rest = [&](int64_t v) -> double {
-    const double e = weight(v);
-    if (plain) return e;
-    if (v == hole) return 0.0;
-    if (!qrow) return e;
-    return v < p.vocab ? fmax(e / Z - (double)qrow[v], 0.0) : 0.0;
-  };
-  double mine;
-  if (plain) {
-    mine = z;
-  } else if (!qrow) {
-    mine = warp_sum_d(holed);
-  } else {
+  const double Z = cluster_total(z, part_z, w, lane, nullptr), inv_z = 1.0 / Z;
+  bool plain = stop >= n;  // the draw is from p itself
+  double mine = warp_sum_d(holed);
+  if (qrow) {
     mine = 0.0;
-    for (int64_t g = g0; g < g1; ++g) mine += rest(g * 32 + lane);
+    for (int i0 = lane; i0 < len; i0 += 32 * kPickBatch) {
+      float q[kPickBatch];
+#pragma unroll
+      for (int k = 0; k < kPickBatch; ++k) q[k] = i0 + 32 * k < len ? __ldg(qrow + v0 + i0 + 32 * k) : 0.f;
+#pragma unroll
+      for (int k = 0; k < kPickBatch; ++k) {
+        const int i = i0 + 32 * k;
+        if (i < len) {
+          const double e = kStored ? kept[i] : weight(v0 + i), rest = fmax(e * inv_z - (double)q[k], 0.0);
+          mine += rest;
+          if (kStored) kept[i] = rest;
+        }
+      }
+    }
     mine = warp_sum_d(mine);
   }
   double before, total = cluster_total(mine, part_r, w, lane, &before);
   if (!plain && !(total > 0.0)) {  // p and q alike in every place: the draw is from p
     plain = true;
-    mine = z;
     total = cluster_total(z, part_p, w, lane, &before);
+    mine = z;
+    if (kStored)
+      for (int i = lane; i < len; i += 32) kept[i] = weight(v0 + i);
   }
+  auto rest_at = [&](int i) -> double {
+    if (kStored) return kept[i];
+    if (plain) return weight(v0 + i);
+    if (v0 + i == hole) return 0.0;
+    const double e = weight(v0 + i);
+    return qrow ? fmax(e * inv_z - (double)qrow[v0 + i], 0.0) : e;
+  };
   const double target = (double)p.uniforms[r1 - 1] * total;
-  // the first index whose running sum passes the target
+  // the first index whose running sum passes the target: in one warp's run, a contiguous piece of it for each lane
   if (before <= target && before + mine > target) {
-    int found = -1, last = -1;
-    double run = before;
-    for (int64_t g = g0; g < g1 && found < 0; ++g) {
-      const int64_t v = g * 32 + lane;
-      const double r = v < p.vocab ? rest(v) : 0.0;
-      double cum = r;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const double y = __shfl_up_sync(0xffffffffu, cum, o);
-        if (lane >= o) cum += y;
-      }
-      const unsigned any = __ballot_sync(0xffffffffu, r > 0.0);
-      const unsigned hit = __ballot_sync(0xffffffffu, r > 0.0 && run + cum > target);
-      if (any) last = (int)(g * 32) + 31 - __clz(any);
-      if (hit) found = (int)(g * 32) + __ffs(hit) - 1;
-      run += __shfl_sync(0xffffffffu, cum, 31);
+    __syncwarp();
+    const int piece = ((len + 31) / 32) | 1;  // (odd: the lanes' pieces start in different banks)
+    const int a = min(lane * piece, len), e = min(a + piece, len);
+    double sum = 0.0;
+    int last = -1;
+    for (int i = a; i < e; ++i) {
+      const double v = rest_at(i);
+      sum += v;
+      if (v > 0.0) last = i;
     }
-    if (found < 0) found = last;  // the sums' last bits
-    if (lane == 0 && found >= 0) atomicMin(&s_found, found);
+    double cum = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double y = __shfl_up_sync(0xffffffffu, cum, o);
+      if (lane >= o) cum += y;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, last >= 0 && before + cum > target);
+    const unsigned any = __ballot_sync(0xffffffffu, last >= 0);
+    // (where the sums' last bits leave no lane: the last index with any weight)
+    const int take = hit ? __ffs(hit) - 1 : (any ? 31 - __clz(any) : -1);
+    if (lane == take) {
+      double at = before + cum - sum;
+      int found = last;
+      for (int i = a; i < e; ++i) {
+        const double v = rest_at(i);
+        at += v;
+        if (v > 0.0 && at > target) {
+          found = i;
+          break;
+        }
+      }
+      atomicMin(&s_found, (int)(v0 + found));
+    }
   }
   cluster_sync_all();
   if (rank == 0 && w == 0) {
@@ -344,9 +384,14 @@ __global__ void __launch_bounds__(kPickThreads) verify_pick_kernel(const VerifyA
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) best = min(best, __shfl_xor_sync(0xffffffffu, best, o));
     if (best == 0x7fffffff) {  // only rounding leaves none: the last index with any weight
-      for (int64_t g = groups - 1; g >= 0 && best == 0x7fffffff; --g) {
+      for (int64_t g = (p.vocab + 31) / 32 - 1; g >= 0 && best == 0x7fffffff; --g) {
         const int64_t v = g * 32 + lane;
-        const unsigned any = __ballot_sync(0xffffffffu, v < p.vocab && rest(v) > 0.0);
+        double rest = 0.0;
+        if (v < p.vocab && v != (plain ? -1 : hole)) {
+          rest = weight(v);
+          if (!plain && qrow) rest = fmax(rest * inv_z - (double)qrow[v], 0.0);
+        }
+        const unsigned any = __ballot_sync(0xffffffffu, rest > 0.0);
         if (any) best = (int)(g * 32) + 31 - __clz(any);
       }
     }
@@ -399,7 +444,20 @@ extern "C" int mg_verify_drafts(const float* logits, int64_t ld, int64_t rows, i
   cudaStream_t st = mg_stream(stream);
   if (rows > 0)
     MG_CUDA_TRY(mg_launch(verify_stats_kernel, dim3((unsigned)a.chunks, (unsigned)rows), dim3(kStatThreads), 0, st, 1, a));
-  MG_CUDA_TRY(mg_launch(verify_pick_kernel, dim3(kPickCtas, (unsigned)b), dim3(kPickThreads), 0, st, kPickCtas, a));
+  // The row's weights are kept in shared memory between the passes while a CTA's eighth of them fits (vocabularies to
+  // 204800); beyond that they are computed again in each.
+  const int64_t nw = kPickCtas * kPickWarps, kept = (vocab + nw - 1) / nw * kPickWarps * (int64_t)sizeof(double);
+  if (kept <= kPickStore) {
+    static bool done[64] = {};
+    static std::mutex mu;
+    MG_CUDA_TRY(mg_once_per_device(done, mu, [] {
+      return cudaFuncSetAttribute(verify_pick_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPickStore);
+    }));
+    MG_CUDA_TRY(mg_launch(verify_pick_kernel<true>, dim3(kPickCtas, (unsigned)b), dim3(kPickThreads), (size_t)kept, st,
+                          kPickCtas, a));
+  } else {
+    MG_CUDA_TRY(mg_launch(verify_pick_kernel<false>, dim3(kPickCtas, (unsigned)b), dim3(kPickThreads), 0, st, kPickCtas, a));
+  }
   MG_LAUNCH_CHECK();
   return MG_OK;
 }

@@ -13,8 +13,10 @@ owns it and passes it back in, as with ``KVCacheState``.
 
 Prefill runs ``prefill_chunk`` positions of every prompt per pass: each INT8 linear
 on all those tokens in one launch (tcgen05 tiles of up to 256 tokens), causal
-attention per prompt on the paged decode kernel (``DecodeEngine.prefill``). Prompts
-that share a leading run of whole
+attention per prompt on the paged decode kernel (``DecodeEngine.prefill``). Padded prompts (an
+attention mask with zeros) and ``prefill_ragged`` pack prompts of different lengths into the
+same passes instead (``DecodeEngine.forward_ragged``), and ``verify`` runs a speculative
+decoding step on them. Prompts that share a leading run of whole
 16-token blocks are prefilled once for that prefix (batch 1) and the blocks are
 shared by reference count; the attention kernel then reads them once per batch.
 With ``prefix_cache_capacity`` > 0 such prefixes are also kept across calls
@@ -216,7 +218,7 @@ class B200QuantizedBackend:
                 cache: Optional[PagedKVCache] = None) -> Tuple[torch.Tensor, PagedKVCache]:
         eng = self._need_model()
         if attention_mask is not None and not bool(torch.as_tensor(attention_mask).bool().all()):
-            raise NotImplementedError("padded prompts are not supported: pass equal-length prompts")
+            return self.prefill_ragged(self._unpadded(input_ids, attention_mask), cache=cache)
         ids = self._ids(input_ids)
         b, T = len(ids), len(ids[0])
         if b > self.max_batch:
@@ -280,6 +282,148 @@ class B200QuantizedBackend:
                     self._run(cache.tables, [r[p] for r in ids], [p] * b, cache.n_shared_blocks,
                               logits=(p == T - 1), cache_mirror=cache.mirror)
             return self._logits_out(b), cache
+
+    @classmethod
+    def _unpadded(cls, input_ids, attention_mask) -> List[List[int]]:
+        """The tokens that a 0/1 attention mask of input_ids' shape keeps, per row (left, right or both padded)."""
+        ids = cls._ids(input_ids)
+        m = torch.as_tensor(attention_mask)
+        keep = (m[None] if m.dim() == 1 else m).bool().cpu()
+        if tuple(keep.shape) != (len(ids), len(ids[0])):
+            raise ValueError(f"a padded batch needs a mask of its own shape {[len(ids), len(ids[0])]}, got "
+                             f"{list(keep.shape)}")
+        rows = []
+        for r, k in zip(ids, keep):
+            at = torch.nonzero(k)[:, 0].tolist()
+            if not at:
+                raise ValueError("a row of the attention mask keeps no token")
+            if at[-1] - at[0] + 1 != len(at):
+                raise ValueError("padding inside a prompt is not supported: only before or behind its tokens")
+            rows.append(r[at[0]:at[-1] + 1])
+        return rows
+
+    def _grow(self, tables: List[BlockTable], counts: List[int]) -> List[int]:
+        """Append ``counts[i]`` token places to every table, all or none; the lengths before."""
+        eng = self._need_model()
+        before = [t.num_tokens for t in tables]
+        if max(n + c for n, c in zip(before, counts)) > eng.max_blocks * BLOCK:
+            raise ValueError(f"a context exceeds max_seq_len {self.max_seq_len}")
+        try:
+            for t, n in zip(tables, counts):
+                for _ in range(n):
+                    self.allocator.append_token(t)
+        except MemoryError:
+            self._shrink(tables, before)
+            raise
+        return before
+
+    def _shrink(self, tables: List[BlockTable], lengths: List[int]) -> None:
+        for t, n in zip(tables, lengths):
+            self.allocator.rollback(t, t.num_tokens - n)
+
+    def prefill_ragged(self, prompts: List[List[int]],
+                       cache: Optional[PagedKVCache] = None) -> Tuple[torch.Tensor, PagedKVCache]:
+        """``prefill`` for prompts of different lengths: every prompt's tokens packed into the same passes, causal
+        attention per prompt (``DecodeEngine.forward_ragged``). Returns (logits [B, V] of each prompt's last token,
+        cache); with ``cache`` the prompts continue its sequences. ``decode`` follows as after ``prefill``."""
+        eng = self._need_model()
+        ids = [[int(t) for t in p] for p in prompts]
+        b = len(ids)
+        if not 0 < b <= self.max_batch:
+            raise ValueError(f"batch {b} > max_batch {self.max_batch}" if b else "no prompt")
+        if any(not p for p in ids):
+            raise ValueError("a prompt needs at least one token")
+        fresh = cache is None or not cache.tables
+        cache = cache or PagedKVCache(self.allocator)
+        tables = [self.allocator.allocate_sequence(f"seq{i}", 0) for i in range(b)] if fresh else cache.tables
+        if len(tables) != b:
+            raise ValueError("cache holds a different batch size")
+        with torch.cuda.device(self._device.torch_device):
+            before = self._grow(tables, [len(p) for p in ids])
+            try:
+                if fresh:
+                    cache.tables, cache.n_shared_blocks = tables, 0
+                if cache.mirror is None or cache.mirror.arr.shape[0] < b:
+                    cache.mirror = TableMirror(b, eng.max_blocks)
+                out = eng.forward_ragged(ids, before, cache.mirror.update(tables))
+                self._greedy = (out, out._version, eng.next_tokens[:b, None].to(torch.int64))
+                K.check_device()
+            except Exception:
+                self._shrink(tables, before)
+                if fresh:
+                    cache.tables = []
+                raise
+            return out, cache
+
+    def verify(self, token_ids: torch.Tensor, drafts, cache: PagedKVCache, draft_probs=None, temperatures=None,
+               uniforms: Optional[torch.Tensor] = None,
+               generator: Optional[torch.Generator] = None) -> Tuple[List[List[int]], PagedKVCache]:
+        """One step of speculative decoding for the whole batch (``SpeculativeEngine``'s target pass and
+        ``rejection_sample_token``, ``scheduler/speculative.py:94-171``): each sequence's last token and its drafted
+        ones run in one packed pass, drafts are accepted by the rejection rule on the device, and the K/V of the
+        others is taken back.
+
+        token_ids [B] or [B, 1]: the token that ``decode`` would be given. drafts: a list of each sequence's drafted
+        tokens (any number, none too) or a tensor [B, k]. draft_probs: the draft's distribution at each drafted place,
+        a list of tensors [k_i, V] or one [B, k, V]; None where the drafts are certain (copied from the prompt, or
+        greedy). temperatures: a number or one per sequence (None = 1, 0 = greedy). uniforms fp32 [sum(k_i + 1)] in
+        [0, 1), drawn with ``generator`` where not given.
+
+        Returns (for every sequence its accepted drafts and the token that follows them, cache). The last of them is
+        the next step's token, as after ``sample``."""
+        eng = self._need_model()
+        if cache is None or not cache.tables:
+            raise ValueError("verify needs the cache returned by prefill")
+        last = torch.as_tensor(token_ids)
+        toks = [r[-1] for r in self._ids(last[:, None] if last.dim() == 1 else last)]
+        dr = [[int(t) for t in d] for d in (drafts.tolist() if torch.is_tensor(drafts) else drafts)]
+        b = len(cache.tables)
+        if len(toks) != b or len(dr) != b:
+            raise ValueError(f"{len(toks)} tokens and {len(dr)} drafts for a cache of {b} sequences")
+        if any(not 0 <= t < self.spec.vocab for d in dr for t in d):
+            raise ValueError("a drafted token is outside the vocabulary")
+        counts = [1 + len(d) for d in dr]
+        R = sum(counts)
+        cu = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
+        dev = self._device.torch_device
+        with torch.cuda.device(dev):
+            probs = None
+            if draft_probs is not None:
+                probs = torch.zeros((R, self.spec.vocab), dtype=torch.float32, device=dev)
+                for i, k in enumerate(len(d) for d in dr):
+                    if k:
+                        pi = torch.as_tensor(draft_probs[i])
+                        if tuple(pi.shape) != (k, self.spec.vocab):
+                            raise ValueError(f"draft_probs of sequence {i} must be [{k}, {self.spec.vocab}]")
+                        probs[int(cu[i]):int(cu[i]) + k] = pi.to(dev)
+            temps = None
+            if temperatures is not None:
+                t = torch.as_tensor(temperatures, dtype=torch.float32).reshape(-1)
+                temps = t.expand(b).contiguous().to(dev) if t.numel() == 1 else t.to(dev)
+            if uniforms is None:
+                uniforms = torch.rand(R, device=dev, generator=generator)
+                if self.world_size > 1:
+                    torch.distributed.broadcast(uniforms, torch.distributed.get_global_rank(self.group, 0)
+                                                if self.group is not None else 0, group=self.group)
+            uniforms = uniforms.to(device=dev, dtype=torch.float32)
+            before = self._grow(cache.tables, counts)
+            try:
+                if cache.mirror is None or cache.mirror.arr.shape[0] < b:
+                    cache.mirror = TableMirror(b, eng.max_blocks)
+                fed = [[t] + d for t, d in zip(toks, dr)]
+                logits = eng.forward_ragged(fed, before, cache.mirror.update(cache.tables), all_logits=True)
+                flat = torch.tensor([t for r in fed for t in r], dtype=torch.int32).to(dev)
+                both = torch.empty((2, b), dtype=torch.int32, device=dev)
+                K.verify_drafts(logits, flat, torch.from_numpy(cu).to(dev), uniforms, draft_probs=probs,
+                                temperatures=temps, accepted=both[0], next_tokens=both[1])
+                K.check_device()
+                acc, nxt = both.tolist()
+            except Exception:
+                self._shrink(cache.tables, before)
+                raise
+            self._shrink(cache.tables, [n + 1 + a for n, a in zip(before, acc)])
+            self._greedy = None
+            return [d[:a] + [t] for d, a, t in zip(dr, acc, nxt)], cache
 
     def _logits_out(self, b: int) -> torch.Tensor:
         """The step's full logits for the caller, remembering the greedy tokens the step already computed

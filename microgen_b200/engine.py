@@ -54,6 +54,8 @@ class LayerWeights:
     d_q: torch.Tensor
     d_s: torch.Tensor
     d_b: Optional[torch.Tensor]
+    qn_w: Optional[torch.Tensor] = None  # RMS norm weights of the query and key heads [head_dim], where the
+    kn_w: Optional[torch.Tensor] = None  # checkpoint has them
 
 
 @dataclass
@@ -198,6 +200,7 @@ class WeightLoader:
                 wd, bd = g(p + "mlp.down_proj.weight"), g(p + "mlp.down_proj.bias")
                 ln1 = (g(p + "input_layernorm.weight"), None)
                 ln2 = (g(p + "post_attention_layernorm.weight"), None)
+            norms = (None, None) if gpt2 else tuple(g(p + f"self_attn.{n}_norm.weight") for n in "qk")
             # column-parallel QKV: each projection quantized whole, then this rank's head rows
             parts_q, parts_s, parts_b = [], [], []
             for w_, b_, n_ in ((wq, bq, qn), (wk, bk, kn), (wv, bv, kn)):
@@ -228,7 +231,8 @@ class WeightLoader:
                 o_q=self.cols(o_q, qn), o_s=o_s, o_b=self.bias(bo),
                 ln2_w=self.f32(ln2[0]), ln2_b=self.bias(ln2[1]),
                 gu_q=gu_q, gu_s=gu_s, gu_b=gu_b,
-                d_q=self.cols(d_q, s.inter), d_s=d_s, d_b=self.bias(bd)))
+                d_q=self.cols(d_q, s.inter), d_s=d_s, d_b=self.bias(bd), qn_w=self.bias(norms[0]),
+                kn_w=self.bias(norms[1])))
         if gpt2:
             embed, wpe = self.f32(state["transformer.wte.weight"]), self.f32(state["transformer.wpe.weight"])
             norm_w, norm_b = self.f32(state["transformer.ln_f.weight"]), self.f32(state["transformer.ln_f.bias"])
@@ -310,6 +314,7 @@ class DecodeEngine:
         self.stage_np = self.stage.numpy()
         self.graphs: dict = {}
         self._pf: Optional[dict] = None  # prefill buffers, sized on first use
+        self._rg: Optional[dict] = None  # ragged-pass buffers and plan, sized on first use
         # MG_STREAMK=1 runs the linears on the stream-K kernel (one wave of CTAs, equal weight bytes each;
         # it needs a zero-filled workspace for partial tiles); the default is the cluster split-K kernel,
         # which measured faster in the decode step (A/B in the same run)
@@ -336,6 +341,8 @@ class DecodeEngine:
         if os.environ.get("MG_BLOCK", "0") != "1" or not isinstance(w.lm_q, K.PackedWeight) or self.pool.quantize:
             return False
         if self.max_batch > K.BLOCK_MAX_TOKENS or s.hidden % 128 or self.D not in (32, 64, 128):
+            return False
+        if any(L.qn_w is not None or L.kn_w is not None for L in w.layers):
             return False
         if world > 1 and self.comm is None:
             return False
@@ -425,6 +432,17 @@ class DecodeEngine:
         else:
             K.rmsnorm(h, w, self.spec.eps, x=x)
 
+    def _append(self, l: int, L: LayerWeights, qkv, positions, slots, q) -> None:
+        """Rotary positions and the K/V append of layer ``l``, with the per-head norms of q and k where the model
+        has them; q goes to ``q`` (in its type)."""
+        if L.qn_w is None and L.kn_w is None and q.dtype == torch.float32:
+            K.rope_kv_append(qkv, positions, self.cos_sin, slots, self.hq, self.hkv, self.D, self.pool.k[l],
+                             self.pool.v[l], q_out=q, **self.pool.scales(l))
+        else:
+            K.norm_rope_kv_append(qkv, positions, self.cos_sin, slots, self.hq, self.hkv, self.D, self.pool.k[l],
+                                  self.pool.v[l], q_weight=L.qn_w, k_weight=L.kn_w, eps=self.spec.eps, q_out=q,
+                                  **self.pool.scales(l))
+
     @staticmethod
     def linear_bytes(q: torch.Tensor, m: int, out_bytes: int, n_out: int) -> int:
         """Algorithmic bytes of one INT8 linear launch: codes + scales + x (bf16) + y."""
@@ -478,9 +496,7 @@ class DecodeEngine:
                 K.i8_linear(x, L.qkv_q, L.qkv_s, L.qkv_b, y=self.qkv[:b], epilogue=K.EPI_STORE_F32,
                             workspace=self.lin_ws)
             with P("rope_kv_append", b * nqkv * 4 + b * self.hq * D * 4 + b * 2 * self.hkv * D * 2):
-                K.rope_kv_append(self.qkv[:b], self.positions[:b], self.cos_sin, self.slots[:b], self.hq,
-                                 self.hkv, self.D, self.pool.k[l], self.pool.v[l], q_out=self.q[:b],
-                                 **self.pool.scales(l))
+                self._append(l, L, self.qkv[:b], self.positions[:b], self.slots[:b], self.q[:b])
             with P("paged_attn", attn_bytes):
                 K.paged_decode_attn(self.q[:b], self.pool.k[l], self.pool.v[l], tab, ctx, self.scale,
                                     n_shared_blocks=n_shared_blocks, out=self.attn[:b], workspace=self.workspace,
@@ -623,8 +639,7 @@ class DecodeEngine:
             for l, Lw in enumerate(w.layers):
                 self._norm(h, Lw.ln1_w, Lw.ln1_b, x)
                 K.i8_linear(x, Lw.qkv_q, Lw.qkv_s, Lw.qkv_b, y=qkv, epilogue=K.EPI_STORE_F32)
-                K.rope_kv_append(qkv, posd, self.cos_sin, slots, self.hq, self.hkv, D, self.pool.k[l],
-                                 self.pool.v[l], q_out=q, **self.pool.scales(l))
+                self._append(l, Lw, qkv, posd, slots, q)
                 for si in range(b):
                     r = slice(si * L, (si + 1) * L)
                     K.paged_decode_attn(q[r], self.pool.k[l], self.pool.v[l], tabd[r], ctx[r], self.scale,
@@ -642,6 +657,135 @@ class DecodeEngine:
                 self.h[:b].copy_(h[L - 1::L])
                 self._norm(self.h[:b], w.norm_w, w.norm_b, self.x[:b])
                 self._head(b, lambda kind, nbytes: contextlib.nullcontext())
+
+    # ---- ragged batches: any number of new tokens per request in one pass -------------------------------
+    RAGGED_ROWS = 2048  # rows of a pass; longer batches take several
+
+    def _ragged_buffers(self, rows: int) -> dict:
+        rg = self._rg
+        if rg is not None and rg["rows"] >= rows:
+            return rg
+        cap = 16
+        while cap < rows:
+            cap *= 2
+        self._rg = None
+        s, dev, H, B, MB = self.spec, self.device, self.spec.hidden, self.max_batch, self.max_blocks
+        n_in = cap + 2 * B + B * MB
+        rg = dict(rows=cap,
+                  h=torch.empty((cap, H), dtype=torch.float32, device=dev),
+                  x=torch.empty((cap, H), dtype=torch.bfloat16, device=dev),
+                  qkv=torch.empty((cap, (self.hq + 2 * self.hkv) * self.D), dtype=torch.float32, device=dev),
+                  q=torch.empty((cap, self.hq, self.D), dtype=torch.bfloat16, device=dev),
+                  attn=torch.empty((cap, self.hq * self.D), dtype=torch.bfloat16, device=dev),
+                  act=torch.empty((cap, self.inter), dtype=torch.bfloat16, device=dev),
+                  inputs=torch.zeros(n_in, dtype=torch.int32, device=dev),
+                  stage=torch.zeros(n_in, dtype=torch.int32, pin_memory=True),
+                  plan=K.RaggedPlan(B, cap, MB, self.hq, self.hkv, self.D, dev))
+        rg["stage_np"] = rg["stage"].numpy()
+        self._rg = rg
+        return rg
+
+    def _ragged_pass(self, tokens, q_lens, ctx, tables: np.ndarray) -> dict:
+        """One pass over ``len(tokens)`` packed rows: request i's next q_lens[i] tokens on top of its ctx[i] cached
+        ones. Leaves the final residual of every row in the returned buffers' ``h``."""
+        s, w = self.spec, self.w
+        R, b, B, MB = len(tokens), len(q_lens), self.max_batch, self.max_blocks
+        rg = self._ragged_buffers(R)
+        torch.cuda.current_stream(self.device).synchronize()  # the staging buffer may still be in flight
+        st, o = rg["stage_np"], rg["rows"]
+        st[:R] = tokens
+        st[o:o + 2 * B] = 0
+        st[o:o + b], st[o + B:o + B + b] = q_lens, ctx
+        tab = st[o + 2 * B:].reshape(B, MB)
+        tab[:b, :tables.shape[1]] = tables
+        tab[:b, tables.shape[1]:] = 0
+        n = o + 2 * B + b * MB
+        inp = rg["inputs"]
+        inp[:n].copy_(rg["stage"][:n], non_blocking=True)
+        plan = K.ragged_plan(rg["plan"], inp[o:o + B], inp[o + B:o + 2 * B], inp[o + 2 * B:].view(B, MB),
+                             self.pool.num_blocks)
+        pos, slots = plan.positions[:R], plan.slots[:R]
+        h, x, qkv, q, attn, act = (rg[k][:R] for k in ("h", "x", "qkv", "q", "attn", "act"))
+        epi_mlp = K.EPI_GELU_BF16 if s.family == "gpt2" else K.EPI_SWIGLU_BF16
+        K.embed(inp[:R], pos, w.embed, w.wpe, h)
+        for l, L in enumerate(w.layers):
+            self._norm(h, L.ln1_w, L.ln1_b, x)
+            K.i8_linear(x, L.qkv_q, L.qkv_s, L.qkv_b, y=qkv, epilogue=K.EPI_STORE_F32)
+            self._append(l, L, qkv, pos, slots, q)
+            K.ragged_attn(q, self.pool.k[l], self.pool.v[l], plan, self.scale, out=attn, **self.pool.scales(l))
+            bias_o = L.o_b if self.rank == 0 else None
+            row_parallel_residual(h, lambda y, e: K.i8_linear(attn, L.o_q, L.o_s, bias_o, y=y, epilogue=e),
+                                  self.rank, self.world, self.group)
+            self._norm(h, L.ln2_w, L.ln2_b, x)
+            K.i8_linear(x, L.gu_q, L.gu_s, L.gu_b, y=act, epilogue=epi_mlp)
+            bias_d = L.d_b if self.rank == 0 else None
+            row_parallel_residual(h, lambda y, e: K.i8_linear(act, L.d_q, L.d_s, bias_d, y=y, epilogue=e),
+                                  self.rank, self.world, self.group)
+        return rg
+
+    def forward_ragged(self, ids, ctx, tables, all_logits: bool = False) -> torch.Tensor:
+        """Run ``ids[i]`` (one or more new tokens) of every request on top of its ``ctx[i]`` cached ones, all requests
+        packed into passes of up to ``RAGGED_ROWS`` rows: the mixture of whole prompts, prompt chunks, single tokens
+        and drafts that the reference runs request by request (``pytorch.py:90-142``, ``scheduler.py:199-226``,
+        ``speculative.py:94-141``). ``tables`` int32 [b, >= ceil((ctx + new) / 16)] already hold the blocks.
+
+        Returns new logits fp32: [b, vocab] of each request's last token (also left, with its greedy token, in
+        ``logits`` / ``next_tokens``), or with ``all_logits`` [sum of new tokens, vocab] of every one."""
+        b = len(ids)
+        lens = [len(r) for r in ids]
+        tab = np.asarray(tables, dtype=np.int32)
+        if not 0 < b <= self.max_batch:
+            raise ValueError(f"{b} requests for a max_batch of {self.max_batch}")
+        if len(ctx) != b or tab.ndim != 2 or tab.shape[0] != b or min(lens) < 1 or min(ctx) < 0:
+            raise ValueError("one context length, one table and at least one new token are needed per request")
+        if tab.shape[1] > self.max_blocks or max(c + n for c, n in zip(ctx, lens)) > 16 * tab.shape[1]:
+            raise ValueError("a block table is too short for its request, or wider than max_seq_len")
+        if self.spec.max_pos and max(c + n for c, n in zip(ctx, lens)) > self.spec.max_pos:
+            raise ValueError(f"the model has {self.spec.max_pos} positions")
+        done, outs = [0] * b, []
+        while any(d < n for d, n in zip(done, lens)):
+            room, take = self.RAGGED_ROWS, []
+            for d, n in zip(done, lens):
+                take.append(min(n - d, room))
+                room -= take[-1]
+            tokens = np.concatenate([np.asarray(r[d:d + t], dtype=np.int32) for r, d, t in zip(ids, done, take)])
+            rg = self._ragged_pass(tokens, take, [c + d for c, d in zip(ctx, done)], tab)
+            R = len(tokens)
+            ends = np.cumsum(take) - 1
+            if all_logits:
+                outs.append((R, take, self._logits_of(rg["h"][:R], rg["x"][:R])))
+            else:
+                last = [i for i in range(b) if take[i] and done[i] + take[i] == lens[i]]
+                if last:
+                    src = torch.as_tensor(ends[last], dtype=torch.long).to(self.device)
+                    dst = torch.as_tensor(last, dtype=torch.long).to(self.device)
+                    self.h.index_copy_(0, dst, rg["h"].index_select(0, src))
+            done = [d + t for d, t in zip(done, take)]
+        if all_logits:
+            if len(outs) == 1:
+                return outs[0][2]
+            parts = [[] for _ in range(b)]  # back into the requests' order
+            for R, take, lg in outs:
+                for i, piece in enumerate(torch.split(lg, take)):
+                    parts[i].append(piece)
+            return torch.cat([p for r in parts for p in r])
+        self._norm(self.h[:b], self.w.norm_w, self.w.norm_b, self.x[:b])
+        self._head(b, lambda kind, nbytes: contextlib.nullcontext())
+        return self.full_logits(b)
+
+    def _logits_of(self, h, x) -> torch.Tensor:
+        """fp32 [rows, vocab] logits of final residual rows ``h`` (``x``: their normed copy's buffer), a new tensor."""
+        w, n = self.w, h.shape[0]
+        self._norm(h, w.norm_w, w.norm_b, x)
+        width = self.logits.shape[1]
+        lg = torch.empty((n, width), dtype=torch.float32, device=self.device)
+        K.i8_linear(x, w.lm_q, w.lm_s, None, y=lg[:, :self.vocab_local], epilogue=K.EPI_STORE_F32)
+        if not self.vocab_parallel:
+            return lg
+        import torch.distributed as dist
+        allv = torch.empty((self.world, n, width), dtype=lg.dtype, device=lg.device)
+        dist.all_gather_into_tensor(allv, lg, group=self.group)
+        return torch.cat([allv[r, :, :e - s_] for r, (s_, e) in enumerate(vocab_bounds(self.spec.vocab, self.world))], 1)
 
     def set_inputs(self, tokens, positions, slots, ctx, tables) -> int:
         """Stage one step's inputs in pinned host memory and copy them to the device input buffer in

@@ -140,7 +140,10 @@ class BatchedScheduler:
     to the allocator."""
 
     def __init__(self, backend, max_batch_size: int = 8, eos_token_id: Optional[int] = None,
-                 pad_token_id: int = 0) -> None:
+                 pad_token_id: int = 0, packed_prefill: bool = False) -> None:
+        """``packed_prefill``: prefill all requests admitted in a step together, whatever their lengths
+        (``backend.prefill_ragged``: one set of passes instead of one per prompt length); prompt prefixes are then
+        not shared."""
         eng = backend._need_model()
         if max_batch_size > eng.max_batch:
             raise ValueError(f"max_batch_size {max_batch_size} > the backend's max_batch {eng.max_batch}")
@@ -148,6 +151,7 @@ class BatchedScheduler:
         self.max_batch_size = max_batch_size
         self.eos_token_id = eos_token_id
         self.pad_token_id = pad_token_id
+        self.packed_prefill = bool(packed_prefill)
         self.request_queue = PriorityQueue()
         self.running_requests: list = []
         self._tables: Dict[str, object] = {}
@@ -273,11 +277,14 @@ class BatchedScheduler:
         done = []
         groups: Dict[int, list] = {}
         for r in new:
-            groups.setdefault(r.num_prompt_tokens, []).append(r)
+            groups.setdefault(0 if self.packed_prefill else r.num_prompt_tokens, []).append(r)
         for reqs in groups.values():
             t0 = time.perf_counter()
-            ids = torch.tensor([list(r.prompt_ids) for r in reqs], dtype=torch.long)
-            logits, cache = self.backend.prefill(ids)
+            if self.packed_prefill:
+                logits, cache = self.backend.prefill_ragged([list(r.prompt_ids) for r in reqs])
+            else:
+                ids = torch.tensor([list(r.prompt_ids) for r in reqs], dtype=torch.long)
+                logits, cache = self.backend.prefill(ids)
             toks = self._sample_rows(reqs, logits)
             self.profiling_stats["backend_cuda_ms"] += (time.perf_counter() - t0) * 1e3
             t0 = time.perf_counter()

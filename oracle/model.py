@@ -148,6 +148,9 @@ class OracleModel:
             q = q.reshape(Hq, D)
             k = k.reshape(Hkv, D)
             v = v.reshape(Hkv, D)
+            if s.family != "gpt2" and p + "self_attn.q_norm.weight" in w:  # per-head norms, before the rotation
+                q = rms_norm(q, f64(w[p + "self_attn.q_norm.weight"]), s.eps)
+                k = rms_norm(k, f64(w[p + "self_attn.k_norm.weight"]), s.eps)
             if s.family != "gpt2":
                 q = q * cos + rotate_half(q) * sin
                 k = k * cos + rotate_half(k) * sin

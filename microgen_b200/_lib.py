@@ -62,7 +62,7 @@ SIGNATURES = {
                                _i64, _p],
     "mg_ragged_attn_workspace_bytes": [_i64, _i, _i, _i, _i, C.POINTER(C.c_size_t)],
     "mg_ragged_attn": [_p, _i64, _p, _p, _p, _p, _i64, _p, _i, _i, _i64, _i, _i, _i, _f, _p, _p, _p, _sz, _p],
-    "mg_verify_workspace_bytes": [_i64, _i64, C.POINTER(C.c_size_t)],
+    "mg_verify_workspace_bytes": [_i64, _i64, _i, C.POINTER(C.c_size_t)],
     "mg_verify_drafts": [_p, _i64, _i64, _i64, _p, _p, _i, _p, _i64, _p, _p, _p, _p, _p, _sz, _p],
     "mg_embed": [_p, _p, _p, _p, _i, _i, _i64, _i, _p, _p],
     "mg_rmsnorm": [_p, _p, _i, _i, _f, _p, _p],

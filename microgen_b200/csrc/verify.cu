@@ -7,12 +7,14 @@
 //   row where every draft was accepted): the first index whose running sum passes u_last times the whole.
 // T = 0 is greedy: d_j is accepted iff it is the row's first maximal index, and that index is the token.
 //
-// Two launches. The first streams every row once and leaves (max, sum of exponentials, argmax) per chunk: bound by
-// memory. The second, one cluster of CTAs per request, decides from those where the request stops, and works on that
-// one row alone. Its sums are in 64 bits: with 10^5 entries the running sum's steps are so close that 32-bit sums
-// put the drawn index one off in about one of a hundred draws, where 64-bit sums of 64-bit exponentials do in none.
-#include <float.h>
-
+// Every row is streamed once by the first launch, which leaves (max, sum of exponentials, argmax) per chunk: bound by
+// memory. The others work on one row per request: they decide from those states where it stops and sum the stopping
+// row's weights by segments (decide), and the sums of max(p - q, 0) where the draft has probabilities (rest); the CTA that
+// sums a request's last segment finds the index in the segment that the target falls into. Small grids that fill the
+// machine measured less (84 us against 103, for 48 requests) than one cluster per request holding the row's weights in
+// shared memory, whose eight CTAs of 128 KB find room a third at a time. The draw's sums are in 64 bits: with 10^5 entries
+// the running sum's steps are so close that 32-bit sums put the drawn index one off in about one of a hundred draws,
+// where 64-bit sums of 64-bit exponentials do in none.
 #include "common.cuh"
 
 namespace {
@@ -20,11 +22,11 @@ namespace {
 constexpr int kStatThreads = 256;
 constexpr int kStatVec = 8;                              // float4 loads in flight per thread
 constexpr int kStatChunk = kStatThreads * 4 * kStatVec;  // logits per CTA
-constexpr int kPickThreads = 512;
-constexpr int kPickWarps = kPickThreads / 32;
-constexpr int kPickCtas = 8;
 constexpr int kPickBatch = 8;                            // loads in flight per thread
-constexpr int kPickStore = 200 * 1024;                   // shared memory for a CTA's share of the weights
+constexpr int kSegments = 16;                            // of the stopping row, one per CTA
+constexpr int kRuns = kSegments * (kStatThreads / 32);   // of the stopping row, one per warp
+
+struct Decision;
 
 struct VerifyArgs {
   const float* logits;
@@ -35,9 +37,19 @@ struct VerifyArgs {
   int64_t vocab;
   int64_t rows;
   int b, chunks;
-  float4* stats;  // [rows][chunks]: max, sum exp((x - max) / T), argmax (bits), unused
+  float4* stats;        // [rows][chunks]: max, sum exp((x - max) / T), argmax (bits), unused
+  Decision* decisions;  // [b]
+  double2* parts;       // [b][runs]: sum of the weights, and of those the one-hot draft leaves
+  double* rest;         // [b][runs]: sum of max(p - q, 0)
+  int32_t* counters;    // [b][2]: segments summed, in the decision and in the rest
   int32_t *accepted, *next;
 };
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 
 // (m, s) <- merge of two (max, sum of exp2((x - max) * c)) states.
 __device__ __forceinline__ void merge_ms(float& m, float& s, float om, float os, float c) {
@@ -53,6 +65,8 @@ __global__ void __launch_bounds__(kStatThreads) verify_stats_kernel(const Verify
   __shared__ int32_t sm_i[kStatThreads / 32];
   const int64_t row = blockIdx.y;
   const int t = threadIdx.x, lane = t & 31, w = t >> 5;
+  if (blockIdx.x == 0 && row == 0)
+    for (int i = t; i < 2 * p.b; i += kStatThreads) p.counters[i] = 0;
   const float* x = p.logits + row * p.ld;
   const int64_t lo = (int64_t)blockIdx.x * kStatChunk, hi = min(lo + (int64_t)kStatChunk, p.vocab);
   float v[4 * kStatVec];
@@ -79,21 +93,25 @@ __global__ void __launch_bounds__(kStatThreads) verify_stats_kernel(const Verify
   float m = -INFINITY, s = 0.f, best = -INFINITY;
   int32_t bi = 0x7fffffff;
   if (T > 0.f) {
+    // the chunk's maximum first: exponentials against it need no rescaling when their sums are joined
     bool nan = false;
 #pragma unroll
     for (int k = 0; k < 4 * kStatVec; ++k) {
       m = fmaxf(m, v[k]);
       nan |= v[k] != v[k];
     }
-    if (m != -INFINITY) {
+    m = warp_max(m);
+    if (lane == 0) sm_m[w] = m;
+    __syncthreads();
 #pragma unroll
-      for (int k = 0; k < 4 * kStatVec; ++k) s += exp2f((v[k] - m) * c);
+    for (int k = 0; k < kStatThreads / 32; ++k) m = fmaxf(m, sm_m[k]);
+    if (m != -INFINITY) {  // (an infinite maximum leaves inf - inf, the NaN that marks the row)
+#pragma unroll
+      for (int k = 0; k < 4 * kStatVec; ++k) s += ex2((v[k] - m) * c);
     }
     if (nan) s = NAN;
-    if (m == -INFINITY && nan) m = 0.f;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
-      merge_ms(m, s, __shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, s, o), c);
+    s = warp_sum(s);
+    if (m == -INFINITY && __syncthreads_or(nan)) m = 0.f;
   } else {
 #pragma unroll
     for (int k = 0; k < kStatVec; ++k)
@@ -116,7 +134,6 @@ __global__ void __launch_bounds__(kStatThreads) verify_stats_kernel(const Verify
     }
   }
   if (lane == 0) {
-    sm_m[w] = m;
     sm_s[w] = s;
     sm_v[w] = best;
     sm_i[w] = bi;
@@ -125,7 +142,7 @@ __global__ void __launch_bounds__(kStatThreads) verify_stats_kernel(const Verify
   if (t == 0) {
     for (int k = 1; k < kStatThreads / 32; ++k) {
       if (T > 0.f) {
-        merge_ms(m, s, sm_m[k], sm_s[k], c);
+        s += sm_s[k];
       } else if (mg_argmax_better(sm_v[k], sm_i[k], best, bi)) {
         best = sm_v[k];
         bi = sm_i[k];
@@ -170,47 +187,165 @@ __device__ __forceinline__ double warp_sum_d(double v) {
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
-__device__ __forceinline__ double ld_dsmem_f64(uint32_t addr) {
-  double v;
-  asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(addr));
+// What the decision leaves for the draw.
+struct __align__(16) Decision {
+  int32_t stop, draw;  // rows kept; 0: answered already, 1: draw from p, 2: draw from what the draft leaves of p
+  float max;           // the stopping row's maximum
+  int32_t pad;
+};
+
+// The stopping row's weights: exp((x - max) / T), and of those max(weight / Z - q, 0) or all but the one-hot draft's.
+struct Row {
+  const float *x, *q;
+  double mx, inv_t, inv_z;
+  int64_t hole;
+  __device__ __forceinline__ double weight(float l) const { return exp(((double)l - mx) * inv_t); }
+  __device__ __forceinline__ double rest(int64_t v) const {
+    const double e = v == hole ? 0.0 : weight(__ldg(x + v));
+    return q ? fmax(e * inv_z - (double)__ldg(q + v), 0.0) : e;
+  }
+};
+__device__ __forceinline__ Row stopping_row(const VerifyArgs& p, const Decision& d, int req, bool rest) {
+  const int64_t r = p.cu[req] + d.stop;
+  Row w;
+  w.x = p.logits + r * p.ld;
+  w.q = rest && p.probs ? p.probs + r * p.ldq : nullptr;
+  w.hole = rest && !p.probs ? (int64_t)p.tokens[r + 1] : -1;
+  w.mx = (double)d.max;
+  w.inv_t = 1.0 / (p.temps ? (double)p.temps[req] : 1.0);
+  w.inv_z = 0.0;
+  return w;
+}
+
+// Run `k` of the vocabulary: [v0, v1).
+__device__ __forceinline__ void run_of(int64_t vocab, int k, int64_t& v0, int64_t& v1) {
+  const int64_t len = (vocab + kRuns - 1) / kRuns;
+  v0 = min((int64_t)k * len, vocab);
+  v1 = min(v0 + len, vocab);
+}
+
+// Inclusive prefix sum of one double per thread over the CTA; red: a double per warp.
+__device__ __forceinline__ double block_prefix(double v, double* red) {
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const double y = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += y;
+  }
+  if (lane == 31) red[w] = v;
+  __syncthreads();
+  for (int k = 0; k < w; ++k) v += red[k];
   return v;
 }
 
-// Sum over the cluster's CTAs and warps of each warp's `mine`, and (before) the sum of those before this warp, in
-// (CTA, warp) order. part: kPickWarps doubles of shared memory, free for reuse after the next cluster barrier.
-__device__ __forceinline__ double cluster_total(double mine, double* part, int w, int lane, double* before) {
-  if (lane == 0) part[w] = mine;
-  cluster_sync_all();
-  const uint32_t rank = cluster_ctarank();
-  double total = 0.0, pre = 0.0;
-#pragma unroll
-  for (int k = lane; k < kPickCtas * kPickWarps; k += 32) {
-    const uint32_t r = (uint32_t)(k / kPickWarps);
-    const double v = ld_dsmem_f64(mapa_shared(smem_u32(part + k % kPickWarps), r));
-    total += v;
-    if ((int)r < (int)rank || (r == rank && k % kPickWarps < w)) pre += v;
+// The draw, by the CTA that sums a request's last segment: the run in which the running sum passes the target, then the
+// index within it, a few entries for each thread.
+__device__ __forceinline__ void draw_index(const VerifyArgs& p, int req, const Decision& d) {
+  static_assert(kRuns <= kStatThreads, "a thread for each run");
+  constexpr int kWarps = kStatThreads / 32;
+  __shared__ double s_red[2][kWarps], s_total, s_before;
+  __shared__ int s_first[2], s_last[2];
+  const int t = threadIdx.x;
+  if (t < 2) {
+    s_first[t] = 0x7fffffff;
+    s_last[t] = -1;
   }
-  if (before) *before = warp_sum_d(pre);
-  return warp_sum_d(total);
+  const double2 z = t < kRuns ? __ldcg(p.parts + (int64_t)req * kRuns + t) : make_double2(0.0, 0.0);
+  bool rest = d.draw == 2;
+  double part = !rest ? z.x : (p.probs ? (t < kRuns ? __ldcg(p.rest + (int64_t)req * kRuns + t) : 0.0) : z.y);
+  if (rest && !__syncthreads_or(part > 0.0)) {  // p and q alike in every place: the draw is from p
+    rest = false;
+    part = z.x;
+  }
+  double Z = z.x;
+  if (rest && p.probs) {  // (the whole of the weights, for p itself)
+    Z = block_prefix(z.x, s_red[0]);
+    if (t == kStatThreads - 1) s_total = Z;
+    __syncthreads();
+    Z = s_total;
+    __syncthreads();
+  }
+  const double cum = block_prefix(part, s_red[1]);
+  if (t == kStatThreads - 1) s_total = cum;
+  __syncthreads();
+  const double target = (double)p.uniforms[p.cu[req + 1] - 1] * s_total;
+  if (part > 0.0) {
+    atomicMax(&s_last[0], t);
+    if (cum > target) atomicMin(&s_first[0], t);
+  }
+  __syncthreads();
+  const int run = s_first[0] != 0x7fffffff ? s_first[0] : s_last[0];  // (the last where the sums' last bits leave none)
+  if (t == run) s_before = cum - part;
+  if (run < 0) {
+    if (t == 0) p.next[req] = -1;
+    return;
+  }
+  Row row = stopping_row(p, d, req, rest);
+  row.inv_z = 1.0 / Z;
+  int64_t v0, v1;
+  run_of(p.vocab, run, v0, v1);
+  const int64_t piece = (v1 - v0 + kStatThreads - 1) / kStatThreads, a = min(v0 + t * piece, v1), e = min(a + piece, v1);
+  double sum = 0.0;
+  int64_t last = -1;
+#pragma unroll 4
+  for (int64_t v = a; v < e; ++v) {
+    const double r = row.rest(v);
+    sum += r;
+    if (r > 0.0) last = v;
+  }
+  const double in = block_prefix(sum, s_red[0]), base = s_before + (in - sum);  // (its barrier covers s_before)
+  if (last >= 0) {
+    atomicMax(&s_last[1], t);
+    if (base + sum > target) atomicMin(&s_first[1], t);
+  }
+  __syncthreads();
+  const int owner = s_first[1] != 0x7fffffff ? s_first[1] : s_last[1];
+  if (t == owner) {
+    double at = base;
+    int64_t found = last;
+    for (int64_t v = a; v < e; ++v) {
+      const double r = row.rest(v);
+      at += r;
+      if (r > 0.0 && at > target) {
+        found = v;
+        break;
+      }
+    }
+    p.next[req] = (int32_t)found;
+  }
+  if (owner < 0 && t == 0) p.next[req] = -1;
 }
 
-template <bool kStored>
-__global__ void __launch_bounds__(kPickThreads) verify_pick_kernel(const VerifyArgs p) {
-  extern __shared__ double weights[];
+// Whether this CTA's segment is the request's last to be summed (its warps have written their sums, each with a fence).
+__device__ __forceinline__ bool last_segment(int32_t* counter) {
+  __shared__ int s_done;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    s_done = atomicAdd(counter, 1) == kSegments - 1;
+    __threadfence();
+  }
+  __syncthreads();
+  return s_done != 0;
+}
+
+// Decides where request blockIdx.y stops (every CTA for itself, from the rows' states), answers it where no draw is
+// needed, and sums one segment of the stopping row: part[0] its weights, part[1] those but the one-hot draft's.
+__global__ void __launch_bounds__(kStatThreads) verify_decide_kernel(const VerifyArgs p) {
   griddep_launch();
   griddep_wait();
-  __shared__ int s_stop, s_bad;
-  __shared__ double part_z[kPickWarps], part_r[kPickWarps], part_p[kPickWarps];
+  constexpr int kWarps = kStatThreads / 32;
+  __shared__ int s_stop, s_bad, s_next;
   __shared__ float s_max;
-  __shared__ int s_found;
-  const int req = (int)blockIdx.y, rank = (int)blockIdx.x;
+  const int req = (int)blockIdx.y, seg = (int)blockIdx.x;
   const int t = threadIdx.x, lane = t & 31, w = t >> 5;
+  Decision* out = p.decisions + req;
   const int64_t r0 = p.cu[req], r1 = p.cu[req + 1];
-  if (r0 < 0 || r1 > p.rows || r1 <= r0) {  // no rows: nothing to ask (the whole cluster leaves together)
-    if (rank == 0 && t == 0) {
+  if (r0 < 0 || r1 > p.rows || r1 <= r0) {  // no rows: nothing to ask
+    if (seg == 0 && t == 0) {
       if (r0 != r1) mg_record_error(MG_ERR_DEVICE, 601);
       p.accepted[req] = 0;
       p.next[req] = -1;
+      out->draw = 0;
     }
     return;
   }
@@ -221,27 +356,28 @@ __global__ void __launch_bounds__(kPickThreads) verify_pick_kernel(const VerifyA
   if (t == 0) {
     s_stop = n;
     s_bad = T < 0.f || T != T ? 602 : 0;
-    s_found = 0x7fffffff;
   }
   __syncthreads();
   // one warp per row: the row's state from its chunks, then the test of its draft
-  for (int j = w; j <= n; j += kPickWarps) {
+  for (int j = w; j <= n; j += kWarps) {
     float m, sum;
-    int32_t bi;
+    int32_t bi, d = -1;
+    float ld = 0.f, qd = 1.f, ud = 0.f;
+    if (j < n && lane == 0) {  // (under way while the chunks are read)
+      d = p.tokens[r0 + j + 1];
+      if (d >= 0 && d < p.vocab) {
+        ld = p.logits[(r0 + j) * p.ld + d];
+        if (p.probs) qd = p.probs[(r0 + j) * p.ldq + d];
+      }
+      ud = p.uniforms[r0 + j];
+    }
     row_state(p.stats + (r0 + j) * p.chunks, p.chunks, lane, greedy, c, m, sum, bi);
     if (lane == 0) {
       bool ok = false;
       if (j < n) {
-        const int32_t d = p.tokens[r0 + j + 1];
-        if (d < 0 || d >= p.vocab) {
-          atomicMax(&s_bad, 603);
-        } else if (greedy) {
-          ok = d == bi;
-        } else {
-          const double pd = exp(((double)p.logits[(r0 + j) * p.ld + d] - (double)m) / (double)T) / (double)sum;
-          const double qd = p.probs ? (double)p.probs[(r0 + j) * p.ldq + d] : 1.0;
-          ok = (double)p.uniforms[r0 + j] * qd < pd;
-        }
+        if (d < 0 || d >= p.vocab) atomicMax(&s_bad, 603);
+        else if (greedy) ok = d == bi;
+        else ok = (double)ud * (double)qd < exp(((double)ld - (double)m) / (double)T) / (double)sum;
       }
       if (!ok) atomicMin(&s_stop, j);
     }
@@ -254,161 +390,104 @@ __global__ void __launch_bounds__(kPickThreads) verify_pick_kernel(const VerifyA
     row_state(p.stats + (r0 + stop) * p.chunks, p.chunks, lane, greedy, c, m, sum, bi);
     if (lane == 0) {
       s_max = m;
+      s_next = bi == 0x7fffffff ? 0 : bi;
       if (!greedy && (m == -INFINITY || m == INFINITY || sum != sum)) atomicMax(&s_bad, 604);
-      if (greedy) s_found = bi == 0x7fffffff ? 0 : bi;
     }
   }
   __syncthreads();
   const int bad = s_bad;
-  if (bad && rank == 0 && t == 0) mg_record_error(MG_ERR_DEVICE, bad);
-  // (every CTA of the cluster has taken the same decisions from the same data)
-  if (greedy || bad == 602 || bad == 604) {
-    if (rank == 0 && t == 0) {
-      p.accepted[req] = bad == 602 ? 0 : stop;
-      p.next[req] = bad == 602 || bad == 604 ? -1 : s_found;
-    }
-    return;
+  const bool answered = greedy || bad == 602 || bad == 604;
+  if (seg == 0 && t == 0) {
+    if (bad) mg_record_error(MG_ERR_DEVICE, bad);
+    p.accepted[req] = bad == 602 ? 0 : stop;
+    if (answered) p.next[req] = bad == 602 || bad == 604 ? -1 : s_next;
+    out->stop = stop;
+    out->max = s_max;
+    out->draw = answered ? 0 : (stop < n ? 2 : 1);
   }
-
-  // ---- draw from the stopping row ----
-  const float* x = p.logits + (r0 + stop) * p.ld;
-  const float* qrow = stop < n && p.probs ? p.probs + (r0 + stop) * p.ldq : nullptr;
-  const int64_t hole = stop < n && !p.probs ? (int64_t)p.tokens[r0 + stop + 1] : -1;  // a one-hot draft's token
-  const double mx = (double)s_max, inv_t = 1.0 / (double)T;
-  // each warp owns a contiguous run of the vocabulary; in the stored form its weights stay in shared memory
-  const int64_t nw = kPickCtas * kPickWarps, run = (p.vocab + nw - 1) / nw;
-  const int64_t me = (int64_t)rank * kPickWarps + w;
-  const int64_t v0 = min(me * run, p.vocab);
-  const int len = (int)(min(v0 + run, p.vocab) - v0);
-  double* kept = weights + (kStored ? (int64_t)w * run : 0);
-  auto weight = [&](int64_t v) -> double { return exp(((double)x[v] - mx) * inv_t); };
-  double z = 0.0, holed = 0.0;
-  for (int i0 = lane; i0 < len; i0 += 32 * kPickBatch) {
+  if (answered) return;
+  Decision d;
+  d.stop = stop;
+  d.draw = stop < n ? 2 : 1;
+  d.max = s_max;
+  const Row row = stopping_row(p, d, req, stop < n && bad != 603 && !p.probs);
+  int64_t v0, v1;
+  run_of(p.vocab, seg * kWarps + w, v0, v1);
+  double z = 0.0, held = 0.0;
+  for (int64_t i0 = v0 + lane; i0 < v1; i0 += 32 * kPickBatch) {
     float l[kPickBatch];
 #pragma unroll
-    for (int k = 0; k < kPickBatch; ++k) l[k] = i0 + 32 * k < len ? __ldg(x + v0 + i0 + 32 * k) : 0.f;
+    for (int k = 0; k < kPickBatch; ++k) l[k] = i0 + k * 32 < v1 ? __ldg(row.x + i0 + k * 32) : 0.f;
 #pragma unroll
     for (int k = 0; k < kPickBatch; ++k) {
-      const int i = i0 + 32 * k;
-      if (i < len) {
-        double e = exp(((double)l[k] - mx) * inv_t);
+      const int64_t v = i0 + k * 32;
+      if (v < v1) {
+        const double e = row.weight(l[k]);
         z += e;
-        if (v0 + i == hole) e = 0.0;  // nothing is left of it
-        holed += e;
-        if (kStored) kept[i] = e;
+        if (v != row.hole) held += e;
       }
     }
   }
   z = warp_sum_d(z);
-  const double Z = cluster_total(z, part_z, w, lane, nullptr), inv_z = 1.0 / Z;
-  bool plain = stop >= n;  // the draw is from p itself
-  double mine = warp_sum_d(holed);
-  if (qrow) {
-    mine = 0.0;
-    for (int i0 = lane; i0 < len; i0 += 32 * kPickBatch) {
-      float q[kPickBatch];
-#pragma unroll
-      for (int k = 0; k < kPickBatch; ++k) q[k] = i0 + 32 * k < len ? __ldg(qrow + v0 + i0 + 32 * k) : 0.f;
-#pragma unroll
-      for (int k = 0; k < kPickBatch; ++k) {
-        const int i = i0 + 32 * k;
-        if (i < len) {
-          const double e = kStored ? kept[i] : weight(v0 + i), rest = fmax(e * inv_z - (double)q[k], 0.0);
-          mine += rest;
-          if (kStored) kept[i] = rest;
-        }
-      }
-    }
-    mine = warp_sum_d(mine);
+  held = warp_sum_d(held);
+  if (lane == 0) {
+    p.parts[(int64_t)req * kRuns + seg * kWarps + w] = make_double2(z, held);
+    __threadfence();
   }
-  double before, total = cluster_total(mine, part_r, w, lane, &before);
-  if (!plain && !(total > 0.0)) {  // p and q alike in every place: the draw is from p
-    plain = true;
-    total = cluster_total(z, part_p, w, lane, &before);
-    mine = z;
-    if (kStored)
-      for (int i = lane; i < len; i += 32) kept[i] = weight(v0 + i);
-  }
-  auto rest_at = [&](int i) -> double {
-    if (kStored) return kept[i];
-    if (plain) return weight(v0 + i);
-    if (v0 + i == hole) return 0.0;
-    const double e = weight(v0 + i);
-    return qrow ? fmax(e * inv_z - (double)qrow[v0 + i], 0.0) : e;
-  };
-  const double target = (double)p.uniforms[r1 - 1] * total;
-  // the first index whose running sum passes the target: in one warp's run, a contiguous piece of it for each lane
-  if (before <= target && before + mine > target) {
-    __syncwarp();
-    const int piece = ((len + 31) / 32) | 1;  // (odd: the lanes' pieces start in different banks)
-    const int a = min(lane * piece, len), e = min(a + piece, len);
-    double sum = 0.0;
-    int last = -1;
-    for (int i = a; i < e; ++i) {
-      const double v = rest_at(i);
-      sum += v;
-      if (v > 0.0) last = i;
-    }
-    double cum = sum;
+  if (d.draw == 2 && p.probs) return;
+  if (last_segment(p.counters + 2 * req)) draw_index(p, req, d);
+}
+
+// Where drafts have probabilities: part[1] of a segment becomes the sum of max(p - q, 0).
+__global__ void __launch_bounds__(kStatThreads) verify_rest_kernel(const VerifyArgs p) {
+  griddep_launch();
+  griddep_wait();
+  constexpr int kWarps = kStatThreads / 32;
+  __shared__ double s_z;
+  const int req = (int)blockIdx.y, seg = (int)blockIdx.x;
+  const int t = threadIdx.x, lane = t & 31, w = t >> 5;
+  const Decision d = p.decisions[req];
+  if (d.draw != 2) return;
+  Row row = stopping_row(p, d, req, true);
+  if (w == 0) {
+    double Z = 0.0;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const double y = __shfl_up_sync(0xffffffffu, cum, o);
-      if (lane >= o) cum += y;
-    }
-    const unsigned hit = __ballot_sync(0xffffffffu, last >= 0 && before + cum > target);
-    const unsigned any = __ballot_sync(0xffffffffu, last >= 0);
-    // (where the sums' last bits leave no lane: the last index with any weight)
-    const int take = hit ? __ffs(hit) - 1 : (any ? 31 - __clz(any) : -1);
-    if (lane == take) {
-      double at = before + cum - sum;
-      int found = last;
-      for (int i = a; i < e; ++i) {
-        const double v = rest_at(i);
-        at += v;
-        if (v > 0.0 && at > target) {
-          found = i;
-          break;
-        }
-      }
-      atomicMin(&s_found, (int)(v0 + found));
-    }
+    for (int k = 0; k < kRuns / 32; ++k) Z += p.parts[(int64_t)req * kRuns + k * 32 + lane].x;
+    Z = warp_sum_d(Z);
+    if (lane == 0) s_z = Z;
   }
-  cluster_sync_all();
-  if (rank == 0 && w == 0) {
-    int best = 0x7fffffff;
-    if (lane < kPickCtas) {
-      uint32_t v;
-      asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(mapa_shared(smem_u32(&s_found), (uint32_t)lane)));
-      best = (int)v;
+  int64_t v0, v1;
+  run_of(p.vocab, seg * kWarps + w, v0, v1);
+  __syncthreads();
+  row.inv_z = 1.0 / s_z;
+  double r = 0.0;
+  for (int64_t i0 = v0 + lane; i0 < v1; i0 += 32 * kPickBatch) {
+    float l[kPickBatch], q[kPickBatch];
+#pragma unroll
+    for (int k = 0; k < kPickBatch; ++k) {
+      const int64_t v = i0 + k * 32;
+      l[k] = v < v1 ? __ldg(row.x + v) : 0.f;
+      q[k] = v < v1 ? __ldg(row.q + v) : 0.f;
     }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) best = min(best, __shfl_xor_sync(0xffffffffu, best, o));
-    if (best == 0x7fffffff) {  // only rounding leaves none: the last index with any weight
-      for (int64_t g = (p.vocab + 31) / 32 - 1; g >= 0 && best == 0x7fffffff; --g) {
-        const int64_t v = g * 32 + lane;
-        double rest = 0.0;
-        if (v < p.vocab && v != (plain ? -1 : hole)) {
-          rest = weight(v);
-          if (!plain && qrow) rest = fmax(rest * inv_z - (double)qrow[v], 0.0);
-        }
-        const unsigned any = __ballot_sync(0xffffffffu, rest > 0.0);
-        if (any) best = (int)(g * 32) + 31 - __clz(any);
-      }
-    }
-    if (lane == 0) {
-      p.accepted[req] = stop;
-      p.next[req] = best == 0x7fffffff ? -1 : best;
-    }
+    for (int k = 0; k < kPickBatch; ++k)
+      if (i0 + k * 32 < v1) r += fmax(row.weight(l[k]) * row.inv_z - (double)q[k], 0.0);
   }
-  cluster_sync_all();  // the other CTAs' results stay readable until rank 0 has read them
+  r = warp_sum_d(r);
+  if (lane == 0) {
+    p.rest[(int64_t)req * kRuns + seg * kWarps + w] = r;
+    __threadfence();
+  }
+  if (last_segment(p.counters + 2 * req + 1)) draw_index(p, req, d);
 }
 
 }  // namespace
 
-extern "C" int mg_verify_workspace_bytes(int64_t rows, int64_t vocab, size_t* bytes) {
-  if (!bytes || rows < 0 || vocab <= 0) return MG_ERR_INVALID_ARG;
-  if (vocab > 0x7fffffc0 || rows > 65535) return MG_ERR_UNSUPPORTED;
-  *bytes = (size_t)rows * (size_t)((vocab + kStatChunk - 1) / kStatChunk) * sizeof(float4);
+extern "C" int mg_verify_workspace_bytes(int64_t rows, int64_t vocab, int b, size_t* bytes) {
+  if (!bytes || rows < 0 || vocab <= 0 || b < 0) return MG_ERR_INVALID_ARG;
+  if (vocab > 0x7fffffc0 || rows > 65535 || b > 65535) return MG_ERR_UNSUPPORTED;
+  *bytes = (size_t)rows * (size_t)((vocab + kStatChunk - 1) / kStatChunk) * sizeof(float4) +
+           (size_t)b * (sizeof(Decision) + kRuns * (sizeof(double2) + sizeof(double)) + 2 * sizeof(int32_t));
   return MG_OK;
 }
 
@@ -417,13 +496,12 @@ extern "C" int mg_verify_drafts(const float* logits, int64_t ld, int64_t rows, i
                                 const float* uniforms, const float* temperatures, int32_t* accepted, int32_t* next,
                                 void* workspace, size_t workspace_bytes, void* stream) {
   size_t need = 0;
-  const int rc = mg_verify_workspace_bytes(rows, vocab, &need);
+  const int rc = mg_verify_workspace_bytes(rows, vocab, b, &need);
   if (rc) return rc;
   if (b < 0 || ld < vocab || (draft_probs && ld_probs < vocab) ||
       (b > 0 && (!cu_rows || !accepted || !next)) || (rows > 0 && (!logits || !tokens || !uniforms)) ||
       workspace_bytes < need || (need && !workspace) || (reinterpret_cast<uintptr_t>(workspace) & 15))
     return MG_ERR_INVALID_ARG;
-  if (b > 65535) return MG_ERR_UNSUPPORTED;
   if (b == 0) return MG_OK;
   VerifyArgs a{};
   a.logits = logits;
@@ -439,25 +517,18 @@ extern "C" int mg_verify_drafts(const float* logits, int64_t ld, int64_t rows, i
   a.b = b;
   a.chunks = (int)((vocab + kStatChunk - 1) / kStatChunk);
   a.stats = static_cast<float4*>(workspace);
+  a.parts = reinterpret_cast<double2*>(a.stats + rows * a.chunks);
+  a.decisions = reinterpret_cast<Decision*>(a.parts + (int64_t)b * kRuns);
+  a.rest = reinterpret_cast<double*>(a.decisions + b);
+  a.counters = reinterpret_cast<int32_t*>(a.rest + (int64_t)b * kRuns);
   a.accepted = accepted;
   a.next = next;
   cudaStream_t st = mg_stream(stream);
   if (rows > 0)
     MG_CUDA_TRY(mg_launch(verify_stats_kernel, dim3((unsigned)a.chunks, (unsigned)rows), dim3(kStatThreads), 0, st, 1, a));
-  // The row's weights are kept in shared memory between the passes while a CTA's eighth of them fits (vocabularies to
-  // 204800); beyond that they are computed again in each.
-  const int64_t nw = kPickCtas * kPickWarps, kept = (vocab + nw - 1) / nw * kPickWarps * (int64_t)sizeof(double);
-  if (kept <= kPickStore) {
-    static bool done[64] = {};
-    static std::mutex mu;
-    MG_CUDA_TRY(mg_once_per_device(done, mu, [] {
-      return cudaFuncSetAttribute(verify_pick_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPickStore);
-    }));
-    MG_CUDA_TRY(mg_launch(verify_pick_kernel<true>, dim3(kPickCtas, (unsigned)b), dim3(kPickThreads), (size_t)kept, st,
-                          kPickCtas, a));
-  } else {
-    MG_CUDA_TRY(mg_launch(verify_pick_kernel<false>, dim3(kPickCtas, (unsigned)b), dim3(kPickThreads), 0, st, kPickCtas, a));
-  }
+  const dim3 segs(kSegments, (unsigned)b);
+  MG_CUDA_TRY(mg_launch(verify_decide_kernel, segs, dim3(kStatThreads), 0, st, 1, a));
+  if (draft_probs) MG_CUDA_TRY(mg_launch(verify_rest_kernel, segs, dim3(kStatThreads), 0, st, 1, a));
   MG_LAUNCH_CHECK();
   return MG_OK;
 }

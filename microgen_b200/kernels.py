@@ -408,9 +408,9 @@ def ragged_attn(q, k_pool, v_pool, plan: RaggedPlan, scale, out=None, k_scales=N
 
 
 @functools.lru_cache(maxsize=256)
-def verify_workspace_bytes(rows: int, vocab: int) -> int:
+def verify_workspace_bytes(rows: int, vocab: int, b: int) -> int:
     n = C.c_size_t(0)
-    _lib.call("mg_verify_workspace_bytes", int(rows), int(vocab), C.byref(n))
+    _lib.call("mg_verify_workspace_bytes", int(rows), int(vocab), int(b), C.byref(n))
     return int(n.value)
 
 
@@ -447,13 +447,15 @@ def verify_drafts(logits, tokens, cu_rows, uniforms, draft_probs=None, temperatu
         raise ValueError("rows of logits and draft_probs must not overlap")
     if temperatures is not None:
         _check(temperatures, "temperatures", f32, dev, (b,))
-    if accepted is None or next_tokens is None:
-        both = torch.empty((2, b), dtype=i32, device=logits.device)
-        accepted = both[0] if accepted is None else accepted
-        next_tokens = both[1] if next_tokens is None else next_tokens
-    _check(accepted, "accepted", i32, dev, (b,))
-    _check(next_tokens, "next_tokens", i32, dev, (b,))
-    ws = verify_workspace_bytes(rows, vocab)
+    if accepted is None:
+        accepted = torch.empty(b, dtype=i32, device=logits.device)
+    else:
+        _check(accepted, "accepted", i32, dev, (b,))
+    if next_tokens is None:
+        next_tokens = torch.empty(b, dtype=i32, device=logits.device)
+    else:
+        _check(next_tokens, "next_tokens", i32, dev, (b,))
+    ws = verify_workspace_bytes(rows, vocab, b)
     if workspace is None or workspace.numel() * workspace.element_size() < ws:
         workspace = torch.empty(ws, dtype=torch.uint8, device=logits.device)
     elif workspace.get_device() != dev or not workspace.is_contiguous():
@@ -462,7 +464,7 @@ def verify_drafts(logits, tokens, cu_rows, uniforms, draft_probs=None, temperatu
              _addr(draft_probs), ldq, uniforms.data_ptr(), _addr(temperatures), accepted.data_ptr(),
              next_tokens.data_ptr(), workspace.data_ptr(), ws)
     if rows and b:
-        _lib.LAUNCHES[0] += 1  # the row statistics, then the decision
+        _lib.LAUNCHES[0] += 1 if draft_probs is None else 2  # row statistics, decision, rest
     return accepted, next_tokens
 
 

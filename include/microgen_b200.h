@@ -305,7 +305,7 @@ int mg_ragged_plan(const int32_t* q_lens, const int32_t* ctx_lens, int b, int64_
  * q_weight / k_weight fp32 [d] (NULL = no norm): y = x * rsqrt(mean(x^2) + eps) * weight over each head; cos_sin as
  * for mg_rope_kv_append (NULL = no rotation); q_out [rows, hq, d] in bf16 (q_bf16 != 0) or fp32. K and V go to
  * slots[i] of the pools: bf16, or with k_scales / v_scales int8 codes and scales as mg_rope_kv_append_kv8 stores
- * them. A row with a negative slot is padding: nothing of it is read or written. A position outside the table
+ * them. A row with a negative slot is padding: nothing is written for it. A position outside the table
  * (site 210) or a slot outside the pool (site 211) is recorded and not written. d in {32, 64, 128}. */
 int mg_norm_rope_kv_append(const void* qkv, int qkv_bf16, int64_t ld_qkv, int64_t rows, const int32_t* positions,
                            const float* cos_sin, int max_pos, const int32_t* slots, const float* q_weight,

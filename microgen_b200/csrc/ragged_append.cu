@@ -14,6 +14,7 @@
 namespace {
 
 constexpr int kAppThreads = 256;
+constexpr int kUnits = 2;  // heads per group of lanes
 
 struct AppendArgs {
   const void* qkv;
@@ -55,97 +56,109 @@ __device__ __forceinline__ uint32_t code4(const float4& a, float s) {
 
 template <int D, bool IN16, bool OUT16, bool Q8>
 __global__ void __launch_bounds__(kAppThreads) norm_rope_append_kernel(const AppendArgs p) {
-  constexpr int L = D / 8;  // lanes per head
+  constexpr int L = D / 8;                     // lanes per head
+  constexpr int kPerCta = kAppThreads / L;     // heads a CTA takes at a time
   griddep_launch();
   griddep_wait();
   const int heads = p.hq + 2 * p.hkv;
-  const int64_t units = p.rows * heads;
-  const int64_t u = ((int64_t)blockIdx.x * kAppThreads + threadIdx.x) / L;
-  const int l = threadIdx.x % L;
-  const bool live = u < units;
-  const int64_t r = live ? u / heads : 0;
-  const int hd = live ? (int)(u - r * heads) : 0;
-  const int slot = live ? p.slots[r] : -1;
-  const bool on = live && slot >= 0;  // slot -1: a padding row, left as it is
-  const int j = 4 * l;
-  float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
-  if (on) {
-    const int64_t at = r * p.ld + (int64_t)hd * D + j;
-    a = load4<IN16>(p.qkv, at);
-    b = load4<IN16>(p.qkv, at + D / 2);
-  }
-  const bool is_q = hd < p.hq, is_k = !is_q && hd < p.hq + p.hkv;
-  const float* w = is_q ? p.qw : (is_k ? p.kw : nullptr);
-  if (p.qw || p.kw) {  // (uniform: every lane takes part in the shuffles)
-    float ss = a.x * a.x + a.y * a.y + a.z * a.z + a.w * a.w + b.x * b.x + b.y * b.y + b.z * b.z + b.w * b.w;
+  const int64_t units = p.rows * heads, u0 = (int64_t)blockIdx.x * (kPerCta * kUnits) + threadIdx.x / L;
+  const int l = threadIdx.x % L, j = 4 * l;
+  // every load that depends on the unit's index alone is issued for all of a thread's units before any is used
+  float4 a[kUnits], b[kUnits];
+  int slot[kUnits], pos[kUnits], hd[kUnits];
+  int64_t row[kUnits];
 #pragma unroll
-    for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    if (w) {
-      const float inv = rsqrtf(ss * (1.f / D) + p.eps);
-      const float4 wa = *reinterpret_cast<const float4*>(w + j), wb = *reinterpret_cast<const float4*>(w + D / 2 + j);
-      a = make_float4(a.x * inv * wa.x, a.y * inv * wa.y, a.z * inv * wa.z, a.w * inv * wa.w);
-      b = make_float4(b.x * inv * wb.x, b.y * inv * wb.y, b.z * inv * wb.z, b.w * inv * wb.w);
-    }
-  }
-  bool ok = on;
-  if (p.cos_sin && on && (is_q || is_k)) {
-    const int pos = p.positions[r];
-    if (pos < 0 || pos >= p.max_pos) {
-      if (l == 0) mg_record_error(MG_ERR_DEVICE, 210);
-      ok = false;
+  for (int k = 0; k < kUnits; ++k) {
+    const int64_t u = u0 + k * kPerCta;
+    const bool live = u < units;
+    row[k] = live ? (u <= 0x7fffffff ? (int64_t)((uint32_t)u / (uint32_t)heads) : u / heads) : 0;
+    hd[k] = live ? (int)(u - row[k] * heads) : 0;
+    slot[k] = live ? __ldg(p.slots + row[k]) : -1;
+    pos[k] = live && p.cos_sin ? __ldg(p.positions + row[k]) : 0;
+    const int64_t at = row[k] * p.ld + (int64_t)hd[k] * D + j;
+    if (live) {
+      a[k] = load4<IN16>(p.qkv, at);
+      b[k] = load4<IN16>(p.qkv, at + D / 2);
     } else {
-      const float* cs = p.cos_sin + (int64_t)pos * D;
-      const float4 c = *reinterpret_cast<const float4*>(cs + j), s = *reinterpret_cast<const float4*>(cs + D / 2 + j);
-      const float4 x = a, y = b;
-      a = make_float4(x.x * c.x - y.x * s.x, x.y * c.y - y.y * s.y, x.z * c.z - y.z * s.z, x.w * c.w - y.w * s.w);
-      b = make_float4(y.x * c.x + x.x * s.x, y.y * c.y + x.y * s.y, y.z * c.z + x.z * s.z, y.w * c.w + x.w * s.w);
+      a[k] = b[k] = make_float4(0.f, 0.f, 0.f, 0.f);
     }
   }
-  float mx = 0.f;
-  if constexpr (Q8) {
-    mx = fmaxf(fmaxf(fmaxf(fabsf(a.x), fabsf(a.y)), fmaxf(fabsf(a.z), fabsf(a.w))),
-               fmaxf(fmaxf(fabsf(b.x), fabsf(b.y)), fmaxf(fabsf(b.z), fabsf(b.w))));
 #pragma unroll
-    for (int o = L / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-  }
-  if (!ok) return;
-  if (is_q) {
-    const int64_t at = (r * p.hq + hd) * D + j;
-    if constexpr (OUT16) {
-      __nv_bfloat16* q = static_cast<__nv_bfloat16*>(p.q_out) + at;
-      store4_bf16(q, a);
-      store4_bf16(q + D / 2, b);
-    } else {
-      float* q = static_cast<float*>(p.q_out) + at;
-      *reinterpret_cast<float4*>(q) = a;
-      *reinterpret_cast<float4*>(q + D / 2) = b;
+  for (int k = 0; k < kUnits; ++k) {
+    const bool on = slot[k] >= 0;  // a negative slot: a padding row (or no unit), left as it is
+    const bool is_q = hd[k] < p.hq, is_k = !is_q && hd[k] < p.hq + p.hkv;
+    const float* w = is_q ? p.qw : (is_k ? p.kw : nullptr);
+    float4 x = a[k], y = b[k];
+    if (p.qw || p.kw) {  // (uniform: every lane takes part in the shuffles)
+      float ss = x.x * x.x + x.y * x.y + x.z * x.z + x.w * x.w + y.x * y.x + y.y * y.y + y.z * y.z + y.w * y.w;
+#pragma unroll
+      for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      if (w) {
+        const float inv = rsqrtf(ss * (1.f / D) + p.eps);
+        const float4 wa = __ldg(reinterpret_cast<const float4*>(w + j)), wb = __ldg(reinterpret_cast<const float4*>(w + D / 2 + j));
+        x = make_float4(x.x * inv * wa.x, x.y * inv * wa.y, x.z * inv * wa.z, x.w * inv * wa.w);
+        y = make_float4(y.x * inv * wb.x, y.y * inv * wb.y, y.z * inv * wb.z, y.w * inv * wb.w);
+      }
     }
-    return;
-  }
-  const int64_t blk = slot >> 4;
-  if (blk >= p.num_blocks) {
-    if (l == 0) mg_record_error(MG_ERR_DEVICE, 211);
-    return;
-  }
-  const int kh = hd - p.hq - (is_k ? 0 : p.hkv);
-  const int64_t row = (blk * p.hkv + kh) * 16 + (slot & 15);
-  if constexpr (Q8) {
-    const float s = fmaxf(__fdiv_rn(mx, 127.f), 1e-8f);
-    uint8_t* dst = static_cast<uint8_t*>(is_k ? p.k_pool : p.v_pool) + row * D + j;
-    *reinterpret_cast<uint32_t*>(dst) = code4(a, s);
-    *reinterpret_cast<uint32_t*>(dst + D / 2) = code4(b, s);
-    if (l == 0) (is_k ? p.k_scales : p.v_scales)[row] = s;
-  } else {
-    __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(is_k ? p.k_pool : p.v_pool) + row * D + j;
-    store4_bf16(dst, a);
-    store4_bf16(dst + D / 2, b);
+    bool ok = on;
+    if (p.cos_sin && on && (is_q || is_k)) {
+      if (pos[k] < 0 || pos[k] >= p.max_pos) {
+        if (l == 0) mg_record_error(MG_ERR_DEVICE, 210);
+        ok = false;
+      } else {
+        const float* cs = p.cos_sin + (int64_t)pos[k] * D;
+        const float4 c = __ldg(reinterpret_cast<const float4*>(cs + j)), s = __ldg(reinterpret_cast<const float4*>(cs + D / 2 + j));
+        const float4 u = x, v = y;
+        x = make_float4(u.x * c.x - v.x * s.x, u.y * c.y - v.y * s.y, u.z * c.z - v.z * s.z, u.w * c.w - v.w * s.w);
+        y = make_float4(v.x * c.x + u.x * s.x, v.y * c.y + u.y * s.y, v.z * c.z + u.z * s.z, v.w * c.w + u.w * s.w);
+      }
+    }
+    float mx = 0.f;
+    if constexpr (Q8) {
+      mx = fmaxf(fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))),
+                 fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w))));
+#pragma unroll
+      for (int o = L / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    }
+    if (!ok) continue;
+    if (is_q) {
+      const int64_t at = (row[k] * p.hq + hd[k]) * D + j;
+      if constexpr (OUT16) {
+        __nv_bfloat16* q = static_cast<__nv_bfloat16*>(p.q_out) + at;
+        store4_bf16(q, x);
+        store4_bf16(q + D / 2, y);
+      } else {
+        float* q = static_cast<float*>(p.q_out) + at;
+        *reinterpret_cast<float4*>(q) = x;
+        *reinterpret_cast<float4*>(q + D / 2) = y;
+      }
+      continue;
+    }
+    const int64_t blk = slot[k] >> 4;
+    if (blk >= p.num_blocks) {
+      if (l == 0) mg_record_error(MG_ERR_DEVICE, 211);
+      continue;
+    }
+    const int kh = hd[k] - p.hq - (is_k ? 0 : p.hkv);
+    const int64_t at = (blk * p.hkv + kh) * 16 + (slot[k] & 15);
+    if constexpr (Q8) {
+      const float s = fmaxf(__fdiv_rn(mx, 127.f), 1e-8f);
+      uint8_t* dst = static_cast<uint8_t*>(is_k ? p.k_pool : p.v_pool) + at * D + j;
+      *reinterpret_cast<uint32_t*>(dst) = code4(x, s);
+      *reinterpret_cast<uint32_t*>(dst + D / 2) = code4(y, s);
+      if (l == 0) (is_k ? p.k_scales : p.v_scales)[at] = s;
+    } else {
+      __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(is_k ? p.k_pool : p.v_pool) + at * D + j;
+      store4_bf16(dst, x);
+      store4_bf16(dst + D / 2, y);
+    }
   }
 }
 
 template <int D, bool IN16, bool OUT16>
 int launch_append(const AppendArgs& a, bool q8, cudaStream_t st) {
-  const int64_t units = a.rows * (a.hq + 2 * a.hkv);
-  const int64_t grid = (units * (D / 8) + kAppThreads - 1) / kAppThreads;
+  const int64_t units = a.rows * (a.hq + 2 * a.hkv), per = (int64_t)kAppThreads / (D / 8) * kUnits;
+  const int64_t grid = (units + per - 1) / per;
   if (grid > 0x7fffffff) return MG_ERR_UNSUPPORTED;
   if (q8)
     MG_CUDA_TRY(mg_launch(norm_rope_append_kernel<D, IN16, OUT16, true>, dim3((unsigned)grid), dim3(kAppThreads), 0,

@@ -721,8 +721,9 @@ __global__ void __launch_bounds__(RagCfg<D, Q8>::kThreads, 1)
             if constexpr (Q8) {
 #pragma unroll
               for (int c = 0; c < kRows; c += 4) {
-                const float4 f = *reinterpret_cast<const float4*>(sc + c);
-                s[c] *= f.x, s[c + 1] *= f.y, s[c + 2] *= f.z, s[c + 3] *= f.w;
+                const ulonglong2 f = *reinterpret_cast<const ulonglong2*>(sc + c);
+                unpair(mul2(pair(s[c], s[c + 1]), f.x), s[c], s[c + 1]);
+                unpair(mul2(pair(s[c + 2], s[c + 3]), f.y), s[c + 2], s[c + 3]);
               }
             }
             const int see = my_pos - key0;  // keys 0 .. see of the tile are this row's
@@ -761,29 +762,43 @@ __global__ void __launch_bounds__(RagCfg<D, Q8>::kThreads, 1)
             const float off = m == -INFINITY ? 0.f : -m * p.scale_log2;
             const uint64_t off2 = pair(off, off);
             uint64_t sum[2] = {l2, 0};
+            auto exponentials = [&](auto masked_tag) {
+              constexpr bool kMasked = decltype(masked_tag)::value;
 #pragma unroll
-            for (int h = 0; h < 4; ++h) {
-              uint32_t pk[16];
+              for (int h = 0; h < 4; ++h) {
+                uint32_t pk[16];
 #pragma unroll
-              for (int c = 0; c < 16; ++c) {
-                const int e = h * 32 + 2 * c;
-                const uint64_t x = fma2(pair(s[e], s[e + 1]), scale2, off2);
-                float a, b;
-                unpair(x, a, b);
-                a = ex2(a);
-                b = ex2(b);
-                const uint64_t y = pair(a, b);
-                sum[c & 1] = add2(sum[c & 1], y);
-                if constexpr (Q8) {  // the value's scale, with nothing of a masked key's
-                  unpair(mul2(y, *reinterpret_cast<const uint64_t*>(sc + kRows + e)), a, b);
-                  if (masked) {
-                    a = e <= see ? a : 0.f;
-                    b = e + 1 <= see ? b : 0.f;
+                for (int c = 0; c < 16; c += 2) {
+                  const int e = h * 32 + 2 * c;
+                  float a[4];
+#pragma unroll
+                  for (int y = 0; y < 2; ++y) {
+                    const uint64_t x = fma2(pair(s[e + 2 * y], s[e + 2 * y + 1]), scale2, off2);
+                    unpair(x, a[2 * y], a[2 * y + 1]);
+                    a[2 * y] = ex2(a[2 * y]);
+                    a[2 * y + 1] = ex2(a[2 * y + 1]);
+                    sum[y] = add2(sum[y], pair(a[2 * y], a[2 * y + 1]));
                   }
+                  if constexpr (Q8) {  // the values' scales, with nothing of a masked key's
+                    const ulonglong2 f = *reinterpret_cast<const ulonglong2*>(sc + kRows + e);
+                    unpair(mul2(pair(a[0], a[1]), f.x), a[0], a[1]);
+                    unpair(mul2(pair(a[2], a[3]), f.y), a[2], a[3]);
+                    if constexpr (kMasked) {
+#pragma unroll
+                      for (int y = 0; y < 4; ++y) a[y] = e + y <= see ? a[y] : 0.f;
+                    }
+                  }
+                  pk[c] = pack_bf16x2(a[0], a[1]);
+                  pk[c + 1] = pack_bf16x2(a[2], a[3]);
                 }
-                pk[c] = pack_bf16x2(a, b);
+                tmem_st16(ts + h * 16, pk);
               }
-              tmem_st16(ts + h * 16, pk);
+            };
+            // (int8: compiled twice, since a test inside the loops would cut them into pieces too short to schedule)
+            if constexpr (Q8) {
+              if (masked) exponentials(std::true_type{}); else exponentials(std::false_type{});
+            } else {
+              exponentials(std::false_type{});
             }
             l2 = add2(sum[0], sum[1]);
             tc_wait_st();

@@ -27,7 +27,6 @@ int mg_sm_count() {
 
 namespace {
 
-constexpr int kPlanThreads = 1024;
 constexpr int kPlanCtas = 8;       // one cluster
 constexpr int kPlanMaxB = 8192;
 constexpr int kBuckets = 1024;     // work-list lengths are ordered to this resolution
@@ -42,32 +41,41 @@ struct PlanArgs {
   RagShape s;
 };
 
-// Exclusive prefix of v over the CTA's threads; `total` gets the sum. red: 33 words of shared memory.
-__device__ __forceinline__ int64_t block_prefix(int64_t v, int64_t* red, int64_t* total) {
+// Exclusive prefixes of N values per thread over the CTA's kT threads, in one round of barriers; total gets the sums.
+// red: N * 33 words of shared memory, free for reuse after the next barrier.
+template <int kT, int N>
+__device__ __forceinline__ void block_prefix(int64_t (&v)[N], int64_t (*red)[33], int64_t (&total)[N]) {
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  int64_t x = v;
+  int64_t x[N];
+#pragma unroll
+  for (int n = 0; n < N; ++n) x[n] = v[n];
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
-    if (lane >= o) x += y;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int64_t y = __shfl_up_sync(0xffffffffu, x[n], o);
+      if (lane >= o) x[n] += y;
+    }
   }
   __syncthreads();
-  if (lane == 31) red[w] = x;
+  if (lane == 31) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) red[n][w] = x[n];
+  }
   __syncthreads();
-  if (w == 0) {
-    const int64_t s = lane < kPlanThreads / 32 ? red[lane] : 0;
-    int64_t y = s;
+  // every warp scans the warps' sums for itself
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    int64_t s = lane < kT / 32 ? red[n][lane] : 0;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int64_t z = __shfl_up_sync(0xffffffffu, y, o);
-      if (lane >= o) y += z;
+      const int64_t z = __shfl_up_sync(0xffffffffu, s, o);
+      if (lane >= o) s += z;
     }
-    red[lane] = y - s;
-    if (lane == 31) red[32] = y;
+    total[n] = __shfl_sync(0xffffffffu, s, 31);
+    const int64_t before = __shfl_sync(0xffffffffu, s, w > 0 ? w - 1 : 0);
+    v[n] = (w > 0 ? before : 0) + x[n] - v[n];
   }
-  __syncthreads();
-  *total = red[32];
-  return red[w] + x - v;
 }
 
 // Item (i, j): tokens [j * tok_item, ...) of request i. Index of the request that owns flat item k (first[] is
@@ -81,9 +89,10 @@ __device__ __forceinline__ int owner(const int32_t* first, int b, int k) {
   return lo;
 }
 
-__global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs p) {
+template <int kT>
+__global__ void __launch_bounds__(kT) plan_kernel(const PlanArgs p) {
   extern __shared__ int32_t sm[];
-  __shared__ int64_t red[33];
+  __shared__ int64_t red[3][33];
   __shared__ int32_t hist[kBuckets];
   __shared__ int s_bad;
   int32_t* cu = sm;                    // [b + 1]
@@ -98,7 +107,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs p) {
   __syncthreads();
 
   // ---- read and scan (every CTA for itself) ----
-  const int per = (p.b + kPlanThreads - 1) / kPlanThreads;
+  const int per = (p.b + kT - 1) / kT;
   const int cursor = p.cursor ? *p.cursor : 0;
   int64_t rows = 0, fresh = 0, items = 0;
   int bad = cursor < 0 ? 501 : 0;
@@ -127,10 +136,10 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs p) {
     ctx[i] = c;
     held[i] = h;
   }
-  int64_t n_rows, n_fresh, n_items;
-  int64_t r0 = block_prefix(rows, red, &n_rows);
-  int64_t f0 = block_prefix(fresh, red, &n_fresh);
-  int64_t i0 = block_prefix(items, red, &n_items);
+  int64_t first3[3] = {rows, fresh, items}, all3[3];
+  block_prefix<kT>(first3, red, all3);
+  const int64_t n_rows = all3[0], n_fresh = all3[1], n_items = all3[2];
+  int64_t r0 = first3[0], f0 = first3[1], i0 = first3[2];
   if (n_rows > p.max_rows) bad = 503;
   if (p.free_blocks && n_fresh > p.n_free - cursor) bad = 504;
   if (bad) atomicMax(&s_bad, bad);
@@ -153,7 +162,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs p) {
   if (s_bad) {
     // an impossible request: an empty plan, tables and free list as they were, and the error word set
     if (t == 0 && rank == 0) mg_record_error(MG_ERR_DEVICE, s_bad);
-    const int64_t g = (int64_t)rank * kPlanThreads + t, step = (int64_t)kPlanCtas * kPlanThreads;
+    const int64_t g = (int64_t)rank * kT + t, step = (int64_t)kPlanCtas * kT;
     for (int64_t i = g; i <= p.b; i += step) {
       p.cu[i] = 0;
       if (i < p.b) {
@@ -177,7 +186,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs p) {
 
   // ---- rank 0: per-request outputs and the work list; the other ranks: rows and new table entries ----
   if (rank == 0) {
-    for (int i = t; i <= p.b; i += kPlanThreads) {
+    for (int i = t; i <= p.b; i += kT) {
       p.cu[i] = cu[i];
       if (i < p.b) {
         const int kv = ctx[i] + cu[i + 1] - cu[i], need = (kv + 15) >> 4;
@@ -196,45 +205,43 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs p) {
       cnt = min(p.s.tok_item, q - tok0);
       return (ctx[seq] + tok0 + cnt + kRagTile - 1) / kRagTile;
     };
-    const int ipt = (n + kPlanThreads - 1) / kPlanThreads;
-    int64_t sum = 0;
+    const int ipt = (n + kT - 1) / kT;
+    int64_t one[1] = {0}, total[1];
     for (int k = t * ipt; k < min(n, (t + 1) * ipt); ++k) {
       int a, c, e;
-      sum += tiles(k, a, c, e);
+      one[0] += tiles(k, a, c, e);
     }
-    int64_t total, dummy;
-    block_prefix(sum, red, &total);
-    // one SM's share; where the entries would run in barely more than one wave, longer shares until they fit it
+    block_prefix<kT>(one, red, total);
+    // one SM's share; where fewer items than SMs would give entries for barely more than one wave, longer shares until
+    // they fit it
     const int64_t slots_all = p.s.max_merges;
-    int64_t share = (total + slots_all - 1) / slots_all;
+    int64_t share = (total[0] + slots_all - 1) / slots_all;
     if (share < 2) share = 2;
-    int64_t mine = 0, entries = 0;
-    for (int tries = 0; tries < 24; ++tries) {
-      mine = 0;
+    for (int tries = 0; n < slots_all && tries < 24; ++tries) {
+      one[0] = 0;
       for (int k = t * ipt; k < min(n, (t + 1) * ipt); ++k) {
         int a, c, e;
-        mine += (tiles(k, a, c, e) + share - 1) / share;
+        one[0] += (tiles(k, a, c, e) + share - 1) / share;
       }
-      block_prefix(mine, red, &entries);
-      if (n >= slots_all || entries <= slots_all) break;
+      block_prefix<kT>(one, red, total);
+      if (total[0] <= slots_all) break;
       share += share / 8 + 1;
     }
-    // entries, merges and partial slots before this thread's items
-    int64_t my_merge = 0, my_slots = 0;
+    // merges and partial slots before this thread's items
+    int64_t two[2] = {0, 0}, both[2];
+    for (int k = t; k < kBuckets; k += kT) hist[k] = 0;
     for (int k = t * ipt; k < min(n, (t + 1) * ipt); ++k) {
       int a, c, e;
       const int64_t parts = (tiles(k, a, c, e) + share - 1) / share;
       if (parts > 1) {
-        ++my_merge;
-        my_slots += parts;
+        ++two[0];
+        two[1] += parts;
       }
     }
-    int64_t n_merge;
-    int64_t merge0 = block_prefix(my_merge, red, &n_merge);
-    int64_t slot0 = block_prefix(my_slots, red, &dummy);
+    block_prefix<kT>(two, red, both);  // (its barriers also separate clearing the buckets from counting into them)
+    int64_t merge0 = two[0], slot0 = two[1];
+    const int64_t n_merge = both[0];
     // counting sort, longest entries first (the order decides only when an entry runs)
-    for (int k = t; k < kBuckets; k += kPlanThreads) hist[k] = 0;
-    __syncthreads();
     auto bucket = [&](int64_t len) { return kBuckets - 1 - (int)(len * (kBuckets - 1) / share); };
     for (int k = t * ipt; k < min(n, (t + 1) * ipt); ++k) {
       int a, c, e;
@@ -242,9 +249,18 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs p) {
       for (int64_t x = 0; x < nt; x += step) atomicAdd(&hist[bucket(min(step, nt - x))], 1);
     }
     __syncthreads();
-    const int64_t cnt = t < kBuckets ? hist[t] : 0;
-    const int64_t off = block_prefix(cnt, red, &entries);
-    if (t < kBuckets) hist[t] = (int32_t)off;
+    constexpr int kPer = kBuckets / kT;  // adjacent buckets of a thread
+    one[0] = 0;
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) one[0] += hist[t * kPer + k];
+    block_prefix<kT>(one, red, total);
+    const int64_t entries = total[0];
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      const int c = hist[t * kPer + k];
+      hist[t * kPer + k] = (int32_t)one[0];
+      one[0] += c;
+    }
     __syncthreads();
     RagItem* list = reinterpret_cast<RagItem*>(p.work + p.s.list_off);
     RagMerge* merges = reinterpret_cast<RagMerge*>(p.work + p.s.merge_off);
@@ -283,7 +299,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs p) {
     }
     return;
   }
-  const int64_t g = (int64_t)(rank - 1) * kPlanThreads + t, step = (int64_t)(kPlanCtas - 1) * kPlanThreads;
+  const int64_t g = (int64_t)(rank - 1) * kT + t, step = (int64_t)(kPlanCtas - 1) * kT;
   for (int64_t r = g; r < p.max_rows; r += step) {
     int pos = 0, slot = -1, seq = -1;
     if (r < n_rows) {
@@ -358,10 +374,17 @@ extern "C" int mg_ragged_plan(const int32_t* q_lens, const int32_t* ctx_lens, in
   static bool done[64] = {};
   static std::mutex mu;
   MG_CUDA_TRY(mg_once_per_device(done, mu, [] {
-    return cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                (5 * kPlanMaxB + 2) * (int)sizeof(int32_t));
+    const int most = (5 * kPlanMaxB + 2) * (int)sizeof(int32_t);
+    cudaError_t e = cudaFuncSetAttribute(plan_kernel<256>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+    return e != cudaSuccess
+               ? e
+               : cudaFuncSetAttribute(plan_kernel<1024>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
   }));
-  MG_CUDA_TRY(mg_launch(plan_kernel, dim3(kPlanCtas), dim3(kPlanThreads), smem, mg_stream(stream), kPlanCtas, a));
+  // Small steps are a chain of barriers, which fewer threads pass faster; large ones have rows and items for many.
+  if (b <= 256 && max_rows <= 4096)
+    MG_CUDA_TRY(mg_launch(plan_kernel<256>, dim3(kPlanCtas), dim3(256), smem, mg_stream(stream), kPlanCtas, a));
+  else
+    MG_CUDA_TRY(mg_launch(plan_kernel<1024>, dim3(kPlanCtas), dim3(1024), smem, mg_stream(stream), kPlanCtas, a));
   MG_LAUNCH_CHECK();
   return MG_OK;
 }

@@ -410,7 +410,7 @@ __global__ void __launch_bounds__(kStatThreads) verify_decide_kernel(const Verif
   d.stop = stop;
   d.draw = stop < n ? 2 : 1;
   d.max = s_max;
-  const Row row = stopping_row(p, d, req, stop < n && bad != 603 && !p.probs);
+  const Row row = stopping_row(p, d, req, stop < n && !p.probs);
   int64_t v0, v1;
   run_of(p.vocab, seg * kWarps + w, v0, v1);
   double z = 0.0, held = 0.0;

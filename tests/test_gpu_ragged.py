@@ -693,6 +693,29 @@ def test_verify_records_what_it_cannot_answer(what, site):
     assert (acc[ok].item(), nxt[ok].item()) == (want[0][ok], want[1][ok])
 
 
+def test_verify_invalid_draft_behind_the_stop():
+    """A drafted token outside the vocabulary behind the place where the request stops is recorded, and changes nothing:
+    the token that was turned down is still not drawn again."""
+    vocab, n = 4, 400
+    logits = torch.zeros((3 * n, vocab), device="cuda")
+    tokens = i32([0, 2, 9] * n)  # the first draft is turned down (u = 1 - 2^-24 > p), the second is no token
+    u = torch.rand(3 * n, generator=torch.Generator(device="cuda").manual_seed(0), device="cuda")
+    u[0::3] = 1 - 2.0 ** -24
+    acc, nxt = K().verify_drafts(logits, tokens, torch.arange(0, 3 * n + 1, 3, dtype=torch.int32, device="cuda"), u)
+    assert errors() == (5, 603)
+    assert (acc == 0).all() and (nxt != 2).all() and set(nxt.tolist()) == {0, 1, 3}
+
+
+def test_verify_at_the_edges_of_the_uniform_numbers():
+    """u = 0 draws the first index with any weight, u = 1 (or a little more) the last."""
+    logits = torch.full((2, 1000), -math.inf, device="cuda")
+    logits[:, 17:900:3] = 0.5
+    for u, want in ((0.0, 17), (1.0, 17 + 3 * 294), (1.5, 17 + 3 * 294)):
+        _, nxt = K().verify_drafts(logits, i32([1, 1]), i32([0, 1, 2]), torch.full((2,), u, device="cuda"))
+        assert nxt.tolist() == [want, want]
+    assert errors()[0] == 0
+
+
 def test_verify_greedy_takes_nan_as_the_maximum():
     logits, tokens, cu, u, _ = verify_case([1], 300, False, 4)
     logits[0, 77] = math.nan

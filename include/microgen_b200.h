@@ -305,8 +305,9 @@ int mg_ragged_plan(const int32_t* q_lens, const int32_t* ctx_lens, int b, int64_
  * q_weight / k_weight fp32 [d] (NULL = no norm): y = x * rsqrt(mean(x^2) + eps) * weight over each head; cos_sin as
  * for mg_rope_kv_append (NULL = no rotation); q_out [rows, hq, d] in bf16 (q_bf16 != 0) or fp32. K and V go to
  * slots[i] of the pools: bf16, or with k_scales / v_scales int8 codes and scales as mg_rope_kv_append_kv8 stores
- * them. A row with a negative slot is padding: nothing is written for it. A position outside the table
- * (site 210) or a slot outside the pool (site 211) is recorded and not written. d in {32, 64, 128}. */
+ * them. A row with a negative slot is padding: nothing is written for it; the other slots of a call are distinct.
+ * A position outside the table (site 210) or a slot outside the pool (site 211) is recorded and not written.
+ * q_out must not overlap qkv. d in {32, 64, 128}. */
 int mg_norm_rope_kv_append(const void* qkv, int qkv_bf16, int64_t ld_qkv, int64_t rows, const int32_t* positions,
                            const float* cos_sin, int max_pos, const int32_t* slots, const float* q_weight,
                            const float* k_weight, float eps, int hq, int hkv, int d, void* q_out, int q_bf16,
@@ -316,7 +317,7 @@ int mg_norm_rope_kv_append(const void* qkv, int qkv_bf16, int64_t ld_qkv, int64_
  * of its block table, whose K/V the step has already appended. q bf16 [rows, hq, d]; pools as for
  * mg_paged_decode_attn (bf16), or _kv8 (int8) when k_scales / v_scales are given; scale > 0; hq/hkv <= 16;
  * b, max_rows, hq, hkv, d, block_tables, max_blocks as given to the mg_ragged_plan call that filled `work`.
- * rows: at least the plan's; rows behind the last request are left as they were. Keys that a row may not see
+ * rows: at least the plan's; rows behind the last request are left as they were. out must not overlap q. Keys that a row may not see
  * and pool entries behind a request's last token do not affect it, whatever they hold. workspace: device
  * scratch of mg_ragged_attn_workspace_bytes() bytes, 16-byte aligned, contents irrelevant: calls that overlap on
  * the GPU need separate ones. Results do not depend on timing. A plan for other sizes (site 510) or a block id

@@ -18,13 +18,29 @@
 //     the unrounded values) and O are fp32. O is rescaled only when a row's maximum grew by more than 2^8 in the
 //     exponentials' scale: until then exponentials up to 2^8 stay far inside the range of fp32 and bf16, and the
 //     final division by the sum removes the common factor.
-// An item that the plan split along the keys leaves (O, maximum, sum) in a workspace slot, and a second kernel
-// merges the slots of each split item in order.
+// A CTA takes several items, dealt out by length, and its K/V and Q loads run ahead into the next one. An item of one row
+// tile (single tokens, short drafts, a prompt's end) gives its K/V tiles to the two warpgroups in turn; the first merges
+// their two states from tensor memory. An item that the plan split along the keys leaves (O, maximum, sum) in a workspace
+// slot, and a second kernel merges the slots of each split item in order.
 //
-// Masked places: scores of keys behind a row's position are replaced before they are used, whatever they are.
-// P is zero there, and 0 * V must be zero too: rows of V behind the item's last key are zeroed in the stage, and a
-// V row that some of a tile's rows may not see is looked over; where one holds an infinity or a NaN, that tile's
-// product is done by the softmax threads, over the keys each row sees.
+// Masked places: scores of keys behind a row's position are replaced before they are used, whatever they are. P is zero
+// there, and 0 * V must be zero too: rows of V behind the item's last key are zeroed in the stage. What an infinity or a
+// NaN in the V of a masked key would leave in the output shows there as one: a piece of work whose output holds any is
+// done over in a second pass, which looks over the V rows that some row may not see, and in a tile with such a value
+// leaves the product to the softmax threads, over the keys each row sees.
+//
+// What bounds it, on a B200 (24/8 heads of 128 unless said; floors at 6.55 TB/s and 1675 TFLOP/s):
+//   * an 8192-token prompt, 400-450 us, 0.92-1.03 PFLOP/s, floor 246: a row tile's cycle is its softmax (2.0 k cycles of
+//     128 x 128 exponentials, two warpgroups sharing 16 exponentials a clock) and then its own two products (1.0 k);
+//     the two row tiles overlap to 3.2 k, where the products of both take 2.05 k and the exponentials 2.05 k. Tried and
+//     slower: the products of each tile from a warp of its own (they interleave, and both softmaxes wait for both; 516 us),
+//     steps of 64 keys with two score buffers (S in halves reads Q twice, and a step's fixed costs come twice; 570), P handed
+//     over in halves (433), a quarter of the exponentials as polynomials on the FMA pipe (no gain within 2 %);
+//   * 32 requests of 5 tokens over 300 to 4000 cached ones, 62 us, floor 35: K and V stream at 6.2 TB/s while they do;
+//     the longest CTA's share is 1.2 times the mean, and the merge takes 6 us;
+//   * 24 packed prompts of 17 to 2047 tokens, 14/2 heads of 64, 66 us: the exponentials alone take 26;
+//   * int8, 16 chunks over up to 6000 cached tokens, 107 us against 72 for the same in bf16: the scales of keys and values,
+//     read from shared memory by every row's thread, take as long as the exponentials.
 #include <type_traits>
 
 #include "ragged.cuh"
@@ -1044,6 +1060,8 @@ extern "C" int mg_ragged_attn(const void* q, int64_t rows, const void* k_pool, c
        reinterpret_cast<uintptr_t>(k_scales) | reinterpret_cast<uintptr_t>(v_scales) | reinterpret_cast<uintptr_t>(work) |
        reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(workspace)) & 15)
     return MG_ERR_INVALID_ARG;
+  // (an item may be read again after it has been written)
+  if (mg_overlap(q, rows * hq * d * 2, out, rows * hq * d * 2)) return MG_ERR_INVALID_ARG;
   RagArgs a{};
   a.rows = rows;
   a.num_blocks = num_blocks;

@@ -348,7 +348,8 @@ def norm_rope_kv_append(qkv, positions, cos_sin, slots, hq, hkv, d, k_pool, v_po
     """Per-head RMS norms of q and k (where a weight fp32 [d] is given), RoPE (where a table is given) and the paged
     K/V append of every row of ``qkv`` (fp32 or bf16 [rows, (hq+2*hkv)*d], unit inner stride). Returns q bf16
     [rows, hq, d] (or ``q_out``, bf16 or fp32). int8 pools store each K and V vector quantized with its scale. Rows
-    whose slot is negative are padding and left alone: with padding rows pass ``q_out``, whose rows then stay."""
+    whose slot is negative are padding and left alone: with padding rows pass ``q_out``, whose rows then stay. The
+    other slots are distinct, and ``q_out`` does not overlap ``qkv``."""
     if not qkv.is_cuda or qkv.dtype not in (torch.float32, torch.bfloat16):
         raise TypeError("qkv must be a CUDA tensor, fp32 or bf16 (the ragged path has no CPU fallback)")
     width = (hq + 2 * hkv) * d
@@ -385,8 +386,8 @@ def norm_rope_kv_append(qkv, positions, cos_sin, slots, hq, hkv, d, k_pool, v_po
 
 def ragged_attn(q, k_pool, v_pool, plan: RaggedPlan, scale, out=None, k_scales=None, v_scales=None):
     """Causal attention of a planned step (``ragged_plan``) over its paged K/V: q bf16 [rows, hq, d], the plan's rows
-    in order (rows behind them are ignored, and stay as they were in a given ``out``); pools bf16, or int8 with
-    scales. Returns bf16 [rows, hq*d]. The step's own K/V must already be in the pools."""
+    in order (rows behind them are ignored, and stay as they were in a given ``out``, which must not overlap q); pools
+    bf16, or int8 with scales. Returns bf16 [rows, hq*d]. The step's own K/V must already be in the pools."""
     if plan.tables is None:
         raise ValueError("the plan has not been filled: call ragged_plan first")
     dev, hq, d = plan.device.index, plan.hq, plan.d

@@ -516,6 +516,25 @@ def test_attention_and_plan_in_a_graph():
         assert (out[sum(ql):] == 3).all()
 
 
+def test_two_steps_at_once_and_the_most_requests():
+    """Steps on two streams, each with a plan of its own; and a plan of as many requests as there may be."""
+    cases = [Case([300, 1, 70], [0, 9000, 500], 24, 8, 128, seed=21), Case([1, 1, 5], [12000, 40, 3000], 24, 8, 128, seed=22)]
+    want = [c.fill().run() for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    got = [[], []]
+    for _ in range(8):
+        for i, (c, s) in enumerate(zip(cases, streams)):
+            with torch.cuda.stream(s):
+                c.fill()
+                got[i].append(c.run())
+    torch.cuda.synchronize()
+    for w, g in zip(want, got):
+        assert all(torch.equal(w, x) for x in g)
+    c = Case([1] * 8192, [i % 3 for i in range(8192)], 3, 1, 32, seed=23).fill()
+    check_attn(c, c.run())
+
+
 def test_attention_refuses_wrong_arguments():
     c = Case([4], [0], 14, 2, 64)
     with pytest.raises(ValueError):
@@ -613,6 +632,49 @@ def test_verify_matches_oracle(vocab, probs):
                                 temperatures=None if temps is None else torch.from_numpy(temps).cuda())
         want = verify_oracle(logits, tokens, cu, u.cpu().numpy(), q, temps)
         assert got[0].tolist() == want[0] and got[1].tolist() == want[1]
+    assert errors()[0] == 0
+
+
+def test_verify_in_a_graph_and_on_two_streams():
+    """A captured verification replayed on other numbers, and two of them at once in workspaces of their own."""
+    cases = [verify_case([3, 0, 6, 1], 50257, probs, 30 + int(probs)) for probs in (False, True)]
+    tok, cu = [i32(c[1]) for c in cases], [i32(c[2]) for c in cases]
+
+    def run(i, **kw):
+        return K().verify_drafts(cases[i][0], tok[i], cu[i], cases[i][3], draft_probs=cases[i][4], **kw)
+
+    def want(i):
+        lg, _, c, u, q = cases[i]
+        return verify_oracle(lg, tok[i].cpu().numpy(), c, u.cpu().numpy(), q, None)
+
+    for i in range(2):
+        acc, nxt = i32([0] * 4), i32([0] * 4)
+        ws = torch.empty(K().verify_workspace_bytes(cases[i][0].shape[0], 50257, 4), dtype=torch.uint8, device="cuda")
+        run(i, accepted=acc, next_tokens=nxt, workspace=ws)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            run(i, accepted=acc, next_tokens=nxt, workspace=ws)
+        for seed in (41, 42, 43):
+            new = verify_case([3, 0, 6, 1], 50257, bool(i), seed + 10 * i)
+            cases[i][0].copy_(new[0])
+            tok[i].copy_(i32(new[1]))
+            cases[i][3].copy_(new[3])
+            if i:
+                cases[i][4].copy_(new[4])
+            ws.fill_(255)  # nothing is kept in it from one call to the next
+            g.replay()
+            assert [acc.tolist(), nxt.tolist()] == list(want(i))
+    expect = [want(i) for i in range(2)]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], [[], []]
+    for _ in range(8):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(run(i))
+    torch.cuda.synchronize()
+    for e, g in zip(expect, got):
+        assert all([a.tolist(), n.tolist()] == list(e) for a, n in g)
     assert errors()[0] == 0
 
 

@@ -87,6 +87,15 @@ def test_attention_refusals(lib):
     assert _attn(lib, hq=34) == UNSUP
 
 
+def test_outputs_over_their_inputs_are_refused(lib):
+    n = 4 * 8 * 64 * 2  # bytes of the default q and out
+    for out in (P, ctypes.c_void_p(P.value + n - 16), ctypes.c_void_p(P.value - n + 16)):
+        assert _attn(lib, out=out) == BAD
+    n = 3 * 8 * 64 * 2  # ... and of the default q_out, at P
+    for qkv in (P, ctypes.c_void_p(P.value + n - 16), ctypes.c_void_p(P.value - 2048)):
+        assert _append(lib, qkv=qkv) == BAD
+
+
 def _verify(lib, rows=3, vocab=11, ld=11, ldq=11, b=2, logits=P, probs=None, ws=P, nbytes=1 << 20):
     return lib.mg_verify_drafts(logits, ld, rows, vocab, P, P, b, probs, ldq, P, None, P, P, ws, nbytes, None)
 

@@ -9,8 +9,8 @@
 // values of the first half and their four rotation partners of the second, so that loads are 16 bytes, the
 // rotation needs no exchange, and a norm or an absolute maximum is a few shuffles. All sums are fp32; the one
 // rounding is the store (q and K/V feed bf16 tensor-core products).
-// Two heads per group of lanes keep enough loads in flight: 8192 rows of 24/8 heads of 128 take 47 us on a B200, 5.4 TB/s
-// of the 6.55 that a copy reaches (55 us with one head and the loads behind the slot's); 160 rows 5 us, the launch.
+// Two heads per group of lanes keep enough loads in flight: 8192 rows of 24/8 heads of 128 take 48 us on a B200, 5.3 TB/s
+// of the 6.55 that a copy reaches (56 us with one head and the loads behind the slot's); 160 rows 5 us, the launch.
 #include "common.cuh"
 
 namespace {

@@ -30,17 +30,19 @@
 // leaves the product to the softmax threads, over the keys each row sees.
 //
 // What bounds it, on a B200 (24/8 heads of 128 unless said; floors at 6.55 TB/s and 1675 TFLOP/s):
-//   * an 8192-token prompt, 400-450 us, 0.92-1.03 PFLOP/s, floor 246: a row tile's cycle is its softmax (2.0 k cycles of
-//     128 x 128 exponentials, two warpgroups sharing 16 exponentials a clock) and then its own two products (1.0 k);
-//     the two row tiles overlap to 3.2 k, where the products of both take 2.05 k and the exponentials 2.05 k. Tried and
-//     slower: the products of each tile from a warp of its own (they interleave, and both softmaxes wait for both; 516 us),
-//     steps of 64 keys with two score buffers (S in halves reads Q twice, and a step's fixed costs come twice; 570), P handed
-//     over in halves (433), a quarter of the exponentials as polynomials on the FMA pipe (no gain within 2 %);
-//   * 32 requests of 5 tokens over 300 to 4000 cached ones, 62 us, floor 35: K and V stream at 6.2 TB/s while they do;
-//     the longest CTA's share is 1.2 times the mean, and the merge takes 6 us;
-//   * 24 packed prompts of 17 to 2047 tokens, 14/2 heads of 64, 66 us: the exponentials alone take 26;
-//   * int8, 16 chunks over up to 6000 cached tokens, 107 us against 72 for the same in bf16: the scales of keys and values,
-//     read from shared memory by every row's thread, take as long as the exponentials.
+//   * an 8192-token prompt, 380-450 us with the clock, 0.92-1.1 PFLOP/s, floor 246: a row tile takes its softmax (2.0 k
+//     cycles, two warpgroups sharing an SM's exponentials) and then its own two products (1.0 k); the two row tiles
+//     overlap to 3.2 k cycles, of which the products of both fill two thirds. Tried and slower: the products of each row
+//     tile from a warp of its own (they interleave, and both softmaxes wait for both; a fifth), steps of 64 keys with two
+//     score buffers (a third), reading the scores from tensor memory twice instead of holding 128 of them (up to a tenth). A part
+//     of the exponentials as polynomials, and the rescaling of O behind them, gained nothing;
+//   * 32 requests of 5 tokens over 300 to 4000 cached ones, 60 us, floor 35: the longest CTA's share is 1.2 times the mean,
+//     and the merge adds 5;
+//   * 24 packed prompts of 18 to 2005 tokens, 14/2 heads of 64, 65 us: the exponentials of whole 128 x 128 tiles, most of
+//     them cut by the diagonal; the products would take 13;
+//   * 16 chunks over up to 3800 cached tokens, bf16, 59 us: two or three short items a CTA, each with an end of its own;
+//     int8, 82: codes to bf16 by one warpgroup (2.0 k cycles a tile) and a softmax of 4.2 k cycles, the scales' products included, in
+//     code that strains the instruction caches (95 while all of it was unrolled, with a row per thread).
 #include <type_traits>
 
 #include "ragged.cuh"
@@ -72,8 +74,8 @@ struct RagCfg {
   static_assert(kSmem <= 232448 - 64, "shared memory");
   static constexpr int kThreads = Q8 ? 512 : 384;
   // registers: a block of 384 threads starts with 168 each, one of 512 with 128; the warpgroups' shares add up to that
-  static constexpr int kSoftRegs = Q8 ? 184 : 208;
-  static constexpr int kOtherRegs = Q8 ? 72 : 88;
+  static constexpr int kSoftRegs = Q8 ? 168 : 208;
+  static constexpr int kOtherRegs = Q8 ? 88 : 88;
   static_assert(2 * kSoftRegs + (kThreads / 128 - 2) * kOtherRegs <= (kThreads / 128) * (Q8 ? 128 : 168), "registers");
   static constexpr uint32_t kO = 256;                              // tensor-memory columns: S0, S1, O0, O1
   // fp32 accumulator, bf16 operands, M = 128; S: K-major B of N = 128; O: MN-major B of N = D
@@ -111,8 +113,10 @@ __device__ __forceinline__ float ex2(float x) {
 }
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
-               "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+               "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+               "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+               "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
                : "memory");
 }
 __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
@@ -124,6 +128,43 @@ __device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
                : "r"(taddr));
+}
+
+// 16 rows at a time, laid out as a product's fragments: lane holds columns 8 g + 2 (lane & 3) and the next one of rows
+// lane / 4 (words 4 g, 4 g + 1) and lane / 4 + 8 (words 4 g + 2, 4 g + 3).
+__device__ __forceinline__ void tmem_ld_frag128(uint32_t taddr, uint32_t (&r)[64]) {
+  asm volatile("tcgen05.ld.sync.aligned.16x256b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12,"
+               "%13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32,"
+               "%33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52,"
+               "%53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%64];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                 "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]),
+                 "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]),
+                 "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]),
+                 "=r"(r[29]), "=r"(r[30]), "=r"(r[31]), "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]),
+                 "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]), "=r"(r[41]), "=r"(r[42]),
+                 "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), "=r"(r[48]), "=r"(r[49]),
+                 "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]), "=r"(r[56]),
+                 "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
+               : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_ld_frag32(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile("tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13,"
+               "%14, %15}, [%16];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                 "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+               : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st_frag32(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile("tcgen05.st.sync.aligned.16x256b.x4.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11,"
+               "%12, %13, %14, %15};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]),
+                 "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]),
+                 "r"(r[14]), "r"(r[15]), "r"(taddr));
+}
+// The same of 16-bit pairs: word 2 g holds columns 8 g + 2 (lane & 3) and the next one of row lane / 4, 2 g + 1 of lane / 4 + 8.
+__device__ __forceinline__ void tmem_st_pairs32(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.16x128b.x4.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::"r"(r[0]),
+                 "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(taddr));
 }
 
 // One lane of a converged warp. The compiler knows that elect.sync leaves a single thread, and issues a tensor-core
@@ -439,7 +480,7 @@ __global__ void __launch_bounds__(RagCfg<D, Q8>::kThreads, 1)
             tc_fence_after();
           };
           const int step = dual ? 2 : 1;
-#pragma unroll
+#pragma unroll (Q8 ? 1 : 2)
           for (int w = 0; w < 2; ++w) {
             const int n = w ? n1 : n0;
             if (n == 0 || !ok) continue;
@@ -460,7 +501,7 @@ __global__ void __launch_bounds__(RagCfg<D, Q8>::kThreads, 1)
             const uint64_t v = v_desc + (uint64_t)((iv % NS) * (C::kTileBytes >> 4));
             ok = bar_wait(&full[iv % NS], (iv / NS) & 1, 516);
             bool k_here = false;
-#pragma unroll
+#pragma unroll (Q8 ? 1 : 2)  // (int8: the less code the better, see above)
             for (int w = 0; w < 2; ++w) {
               const int last = dual ? tiles : (w ? n1 : n0);
               if (!ok || (dual ? w != (j & 1) : j >= last)) continue;
@@ -534,7 +575,7 @@ __global__ void __launch_bounds__(RagCfg<D, Q8>::kThreads, 1)
                 // a block that is not in the pool is read as the pool's first (its error has been recorded)
                 const int row = (good ? id : 0) * p.hkv + wk.head;
                 if (elect_one()) mbar_arrive_expect_tx(&cfull[s], (uint32_t)(nb * 16 * (D + 4)));
-#pragma unroll
+#pragma unroll 1
                 for (int y = 0; y < 8; ++y) {
                   const int64_t r = (int64_t)__shfl_sync(0xffffffffu, row, y) * 16;
                   if (y < nb && elect_one()) {
@@ -631,21 +672,32 @@ __global__ void __launch_bounds__(RagCfg<D, Q8>::kThreads, 1)
               if (!ok) break;
               const uint8_t* src = smem + C::kCodes + sc * C::kCodeBytes;
               uint8_t* dst = smem + C::kRing + s * C::kTileBytes;
+              // (a batch's loads before its stores: the compiler cannot tell the two buffers apart; and few batches unrolled,
+              // for the instruction caches)
+              const float scale = reinterpret_cast<const float*>(smem + C::kCodeScales)[sc * kRows + t];
+              constexpr int kBatch = kPer < 2 ? kPer : 2;
+#pragma unroll 1
+              for (int x0 = 0; x0 < kPer; x0 += kBatch) {
+                uint4 c[kBatch];
 #pragma unroll
-              for (int x = 0; x < kPer; ++x) {
-                const int piece = x * 128 + t, r = piece / kParts, q = (piece % kParts) * 2;
-                uint4 c = make_uint4(0, 0, 0, 0);
-                if (r < keys) c = *reinterpret_cast<const uint4*>(src + piece * 16);
-                uint4 lo, hi;
-                i8x4_to_bf16x4(c.x, lo.x, lo.y);
-                i8x4_to_bf16x4(c.y, lo.z, lo.w);
-                i8x4_to_bf16x4(c.z, hi.x, hi.y);
-                i8x4_to_bf16x4(c.w, hi.z, hi.w);
-                *reinterpret_cast<uint4*>(dst + chunk_at<D>(r, q)) = lo;
-                *reinterpret_cast<uint4*>(dst + chunk_at<D>(r, q + 1)) = hi;
+                for (int x = 0; x < kBatch; ++x) c[x] = *reinterpret_cast<const uint4*>(src + ((x0 + x) * 128 + t) * 16);
+#pragma unroll
+                for (int x = 0; x < kBatch; ++x) {
+                  const int piece = (x0 + x) * 128 + t, r = piece / kParts, q = (piece % kParts) * 2;
+                  if (r >= keys) c[x] = make_uint4(0, 0, 0, 0);
+                  uint4 lo, hi;
+                  i8x4_to_bf16x4(c[x].x, lo.x, lo.y);
+                  i8x4_to_bf16x4(c[x].y, lo.z, lo.w);
+                  i8x4_to_bf16x4(c[x].z, hi.x, hi.y);
+                  i8x4_to_bf16x4(c[x].w, hi.z, hi.w);
+                  // (a row's second 128 bytes lie on the banks of its first: those threads store the other way round)
+                  const int swap = (q >> 3) & 1;
+                  *reinterpret_cast<uint4*>(dst + chunk_at<D>(r, q + swap)) = swap ? hi : lo;
+                  *reinterpret_cast<uint4*>(dst + chunk_at<D>(r, q + 1 - swap)) = swap ? lo : hi;
+                }
               }
               scales[(tile % C::kScaleRing) * 2 * kRows + kv * kRows + t] =
-                  t < keys ? reinterpret_cast<const float*>(smem + C::kCodeScales)[sc * kRows + t] : 0.f;
+                  t < keys ? scale : 0.f;
               fence_async_smem();
               __syncwarp();
               if (lane == 0) {
@@ -670,6 +722,10 @@ __global__ void __launch_bounds__(RagCfg<D, Q8>::kThreads, 1)
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t ts = tmem + lane_base + (uint32_t)(w * kRows), to = tmem + lane_base + C::kO + (uint32_t)(w * D);
     const uint64_t scale2 = pair(p.scale_log2, p.scale_log2);
+    constexpr int kR = Q8 ? 4 : 1;  // rows whose maximum and sum the thread holds: t, or as fragments lane / 4 + 8 k
+    [[maybe_unused]] int frag_tok[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) frag_tok[k] = ((t & ~31) + (lane >> 2) + 8 * k) / p.group;
     bool ok = true;
     int base = 0, cs = 0, co = 0, looks = 0, duals = 0, tile0 = 0;
     RagWalk walk;
@@ -688,8 +744,13 @@ __global__ void __launch_bounds__(RagCfg<D, Q8>::kThreads, 1)
         const bool warp_on = (warp & 3) * 32 < valid;
         const int n = w ? wk.n1 : wk.n0;
         if (kAgain && t == 0) odd_v[w] = 0;
-        float m = -INFINITY;  // the maximum in use, in score units
-        uint64_t l2 = 0;      // the sum, in two halves
+        float mr[kR];     // the maxima in use of the thread's rows, in score units
+        uint64_t lr[kR];  // the sums, in two halves
+#pragma unroll
+        for (int k = 0; k < kR; ++k) {
+          mr[k] = -INFINITY;
+          lr[k] = 0;
+        }
         for (int i = 0; i < n && ok; ++i) {
           const int j = wk.dual ? 2 * i + w : i;
           const int key0 = (it.kt0 + j) * kRows;
@@ -728,58 +789,157 @@ __global__ void __launch_bounds__(RagCfg<D, Q8>::kThreads, 1)
             }
           }
           if (warp_on) {
-            float s[kRows];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) tmem_ld32(ts + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&s[c * 32]));
-            tc_wait_ld();
-            [[maybe_unused]] const float* sc =
-                reinterpret_cast<const float*>(smem + C::kScales) + ((tile0 + j) % C::kScaleRing) * 2 * kRows;
             if constexpr (Q8) {
+              // The scales are one per key and the same for every row: with a row per thread, each would read all of
+              // them, and hold 128 scores besides. As fragments a thread has four rows of 32 keys, and works on two of
+              // them at a time; four lanes share a row's maximum and sum.
+              const uint64_t* sc = reinterpret_cast<const uint64_t*>(
+                  reinterpret_cast<const float*>(smem + C::kScales) + ((tile0 + j) % C::kScaleRing) * 2 * kRows) + (lane & 3);
+              auto half = [&](uint32_t down, auto masked_tag) {
+                constexpr bool kMasked = decltype(masked_tag)::value;
+                uint32_t raw[64];
+                tmem_ld_frag128(ts + down, raw);
+                tc_wait_ld();
+                auto at = [&](int k, int g, int e) -> float& {  // row k of the two, key 8 g + 2 (lane & 3) + e
+                  return reinterpret_cast<float&>(raw[4 * g + 2 * k + e]);
+                };
 #pragma unroll
-              for (int c = 0; c < kRows; c += 4) {
-                const ulonglong2 f = *reinterpret_cast<const ulonglong2*>(sc + c);
-                unpair(mul2(pair(s[c], s[c + 1]), f.x), s[c], s[c + 1]);
-                unpair(mul2(pair(s[c + 2], s[c + 3]), f.y), s[c + 2], s[c + 3]);
-              }
-            }
-            const int see = my_pos - key0;  // keys 0 .. see of the tile are this row's
-            if (masked) {
+                for (int g = 0; g < 16; ++g) {
+                  const uint64_t f = sc[4 * g];
 #pragma unroll
-              for (int h = 0; h < kRows; h += 32) {
-                if (key0 + h + 31 > first_pos) {
+                  for (int k = 0; k < 2; ++k) unpair(mul2(pair(at(k, g, 0), at(k, g, 1)), f), at(k, g, 0), at(k, g, 1));
+                }
+                int see[2];  // keys 8 g + e with 8 g + e <= see are the row's
+                bool grow[2];
+                float m_new[2];
 #pragma unroll
-                  for (int c = h; c < h + 32; ++c) s[c] = c <= see ? s[c] : -INFINITY;
+                for (int k = 0; k < 2; ++k) {
+                  see[k] = first_pos + frag_tok[k] - key0 - 2 * (lane & 3);
+                  const float m = mr[k];
+                  float a = m, b = m;
+#pragma unroll
+                  for (int g = 0; g < 16; ++g) {
+                    if constexpr (kMasked) {
+                      at(k, g, 0) = 8 * g <= see[k] ? at(k, g, 0) : -INFINITY;
+                      at(k, g, 1) = 8 * g + 1 <= see[k] ? at(k, g, 1) : -INFINITY;
+                    }
+                    (g & 1 ? b : a) = max3(g & 1 ? b : a, at(k, g, 0), at(k, g, 1));
+                  }
+                  a = fmaxf(a, b);
+                  a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 1));
+                  a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 2));
+                  grow[k] = m == -INFINITY || (a - m) * p.scale_log2 > 8.f;
+                  m_new[k] = grow[k] ? a : m;
+                }
+                if (i > 0 && __any_sync(0xffffffffu, grow[0] || grow[1])) {
+                  float f[2];
+#pragma unroll
+                  for (int k = 0; k < 2; ++k) {
+                    const float m = mr[k];
+                    f[k] = m == -INFINITY ? 0.f : ex2((m - m_new[k]) * p.scale_log2);
+                    lr[k] = mul2(lr[k], pair(f[k], f[k]));
+                  }
+#pragma unroll 1
+                  for (int c = 0; c < D; c += 32) {
+                    uint32_t o[16];
+                    tmem_ld_frag32(to + down + c, o);
+                    tc_wait_ld();
+#pragma unroll
+                    for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f[(x >> 1) & 1]);
+                    tmem_st_frag32(to + down + c, o);
+                  }
+                }
+                uint64_t off2[2];
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                  mr[k] = m_new[k];
+                  const float off = m_new[k] == -INFINITY ? 0.f : -m_new[k] * p.scale_log2;
+                  off2[k] = pair(off, off);
+                }
+#pragma unroll
+                for (int g0 = 0; g0 < 16; g0 += 4) {
+                  uint32_t pk[8];
+#pragma unroll
+                  for (int g = g0; g < g0 + 4; ++g) {
+                    const uint64_t f = sc[kRows / 2 + 4 * g];
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                      float a, b;
+                      unpair(fma2(pair(at(k, g, 0), at(k, g, 1)), scale2, off2[k]), a, b);
+                      a = ex2(a);
+                      b = ex2(b);
+                      lr[k] = add2(lr[k], pair(a, b));
+                      unpair(mul2(pair(a, b), f), a, b);
+                      if constexpr (kMasked) {  // (nothing of a masked key's scale, whatever it is)
+                        a = 8 * g <= see[k] ? a : 0.f;
+                        b = 8 * g + 1 <= see[k] ? b : 0.f;
+                      }
+                      pk[2 * (g - g0) + k] = pack_bf16x2(a, b);
+                    }
+                  }
+                  tmem_st_pairs32(ts + down + g0 * 4, pk);
+                }
+              };
+              // (compiled twice, since tests inside the loops would cut them into pieces too short to schedule; and once for
+              // both halves, which take turns in the same registers: unrolled, the code does not stay in the
+              // instruction caches)
+#pragma unroll 1
+              for (int h = 0; h < 2; ++h) {
+                if (masked) half((uint32_t)(16 * h) << 16, std::true_type{});
+                else half((uint32_t)(16 * h) << 16, std::false_type{});
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                  const float m = mr[k];
+                  const uint64_t l = lr[k];
+                  const int tok = frag_tok[k];
+                  mr[k] = mr[k + 2], mr[k + 2] = m;
+                  lr[k] = lr[k + 2], lr[k + 2] = l;
+                  frag_tok[k] = frag_tok[k + 2], frag_tok[k + 2] = tok;
                 }
               }
-            }
-            float mx[4] = {m, m, m, m};
+            } else {
+              float& m = mr[0];
+              uint64_t& l2 = lr[0];
+              float s[kRows];
 #pragma unroll
-            for (int c = 0; c < kRows; c += 8) {
+              for (int c = 0; c < 4; ++c) tmem_ld32(ts + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&s[c * 32]));
+              tc_wait_ld();
+              const int see = my_pos - key0;  // keys 0 .. see of the tile are this row's
+              if (masked) {
 #pragma unroll
-              for (int x = 0; x < 4; ++x) mx[x] = max3(mx[x], s[c + x], s[c + 4 + x]);
-            }
-            float m_new = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-            const bool grow = m == -INFINITY || (m_new - m) * p.scale_log2 > 8.f;
-            if (!grow) m_new = m;
-            if (i > 0 && __any_sync(0xffffffffu, grow)) {
-              const float f = m == -INFINITY ? 0.f : ex2((m - m_new) * p.scale_log2);
-              l2 = mul2(l2, pair(f, f));
-#pragma unroll 1
-              for (int c = 0; c < D; c += 32) {
-                uint32_t o[32];
-                tmem_ld32(to + c, o);
-                tc_wait_ld();
+                for (int h = 0; h < kRows; h += 32) {
+                  if (key0 + h + 31 > first_pos) {
 #pragma unroll
-                for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
-                tmem_st32(to + c, o);
+                    for (int c = h; c < h + 32; ++c) s[c] = c <= see ? s[c] : -INFINITY;
+                  }
+                }
               }
-            }
-            m = m_new;
-            const float off = m == -INFINITY ? 0.f : -m * p.scale_log2;
-            const uint64_t off2 = pair(off, off);
-            uint64_t sum[2] = {l2, 0};
-            auto exponentials = [&](auto masked_tag) {
-              constexpr bool kMasked = decltype(masked_tag)::value;
+              float mx[4] = {m, m, m, m};
+#pragma unroll
+              for (int c = 0; c < kRows; c += 8) {
+#pragma unroll
+                for (int x = 0; x < 4; ++x) mx[x] = max3(mx[x], s[c + x], s[c + 4 + x]);
+              }
+              float m_new = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+              const bool grow = m == -INFINITY || (m_new - m) * p.scale_log2 > 8.f;
+              if (!grow) m_new = m;
+              if (i > 0 && __any_sync(0xffffffffu, grow)) {
+                const float f = m == -INFINITY ? 0.f : ex2((m - m_new) * p.scale_log2);
+                l2 = mul2(l2, pair(f, f));
+#pragma unroll 1
+                for (int c = 0; c < D; c += 32) {
+                  uint32_t o[32];
+                  tmem_ld32(to + c, o);
+                  tc_wait_ld();
+#pragma unroll
+                  for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
+                  tmem_st32(to + c, o);
+                }
+              }
+              m = m_new;
+              const float off = m == -INFINITY ? 0.f : -m * p.scale_log2;
+              const uint64_t off2 = pair(off, off);
+              uint64_t sum[2] = {l2, 0};
 #pragma unroll
               for (int h = 0; h < 4; ++h) {
                 uint32_t pk[16];
@@ -795,32 +955,17 @@ __global__ void __launch_bounds__(RagCfg<D, Q8>::kThreads, 1)
                     a[2 * y + 1] = ex2(a[2 * y + 1]);
                     sum[y] = add2(sum[y], pair(a[2 * y], a[2 * y + 1]));
                   }
-                  if constexpr (Q8) {  // the values' scales, with nothing of a masked key's
-                    const ulonglong2 f = *reinterpret_cast<const ulonglong2*>(sc + kRows + e);
-                    unpair(mul2(pair(a[0], a[1]), f.x), a[0], a[1]);
-                    unpair(mul2(pair(a[2], a[3]), f.y), a[2], a[3]);
-                    if constexpr (kMasked) {
-#pragma unroll
-                      for (int y = 0; y < 4; ++y) a[y] = e + y <= see ? a[y] : 0.f;
-                    }
-                  }
                   pk[c] = pack_bf16x2(a[0], a[1]);
                   pk[c + 1] = pack_bf16x2(a[2], a[3]);
                 }
                 tmem_st16(ts + h * 16, pk);
               }
-            };
-            // (int8: compiled twice, since a test inside the loops would cut them into pieces too short to schedule)
-            if constexpr (Q8) {
-              if (masked) exponentials(std::true_type{}); else exponentials(std::false_type{});
-            } else {
-              exponentials(std::false_type{});
+              l2 = add2(sum[0], sum[1]);
             }
-            l2 = add2(sum[0], sum[1]);
             tc_wait_st();
             if constexpr (kAgain) {
               if (by_hand) {
-                values_by_hand<D>(smem + C::kRing + ((base + 2 * j + 1) % NS) * C::kTileBytes, ts, to, see, i > 0);
+                values_by_hand<D>(smem + C::kRing + ((base + 2 * j + 1) % NS) * C::kTileBytes, ts, to, my_pos - key0, i > 0);
               }
             }
           }
@@ -833,9 +978,23 @@ __global__ void __launch_bounds__(RagCfg<D, Q8>::kThreads, 1)
         tile0 += wk.tiles;
         if (!ok) break;
         // ---------------- epilogue ----------------
-        float la, lb;
-        unpair(l2, la, lb);
-        float l = la + lb, ml = m == -INFINITY ? -INFINITY : m * p.scale_log2;
+        float l = 0.f, ml = -INFINITY;  // of row t
+#pragma unroll
+        for (int k = 0; k < kR; ++k) {
+          float a, b, m = mr[k];
+          unpair(lr[k], a, b);
+          a += b;
+          if constexpr (Q8) {  // from the fragments' rows
+            a += __shfl_xor_sync(0xffffffffu, a, 1);
+            a += __shfl_xor_sync(0xffffffffu, a, 2);
+            a = __shfl_sync(0xffffffffu, a, (lane & 7) * 4);
+            m = __shfl_sync(0xffffffffu, m, (lane & 7) * 4);
+          }
+          if (!Q8 || k == lane >> 3) {
+            l = a;
+            ml = m == -INFINITY ? -INFINITY : m * p.scale_log2;
+          }
+        }
         const bool both = wk.dual && wk.n1 > 0;  // two states of the same rows: the first warpgroup merges them
         float2* mls = reinterpret_cast<float2*>(smem + C::kMl);
         if (both && w == 1) {

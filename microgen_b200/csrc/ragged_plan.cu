@@ -11,7 +11,7 @@
 // lengths and scans them for itself instead of waiting for another CTA's scan, rank 0 builds the work list while
 // the others write the rows, and one cluster barrier separates reading the inputs from writing the outputs,
 // which may therefore alias them (a loop feeds held-block counts, the cursor and lengths back in).
-// On a B200: 9.5 us for 32 requests, 15 for 1000 prompts of 57 thousand rows.
+// On a B200: 9 us for 32 requests, 15 for 1000 prompts of 53 thousand rows.
 #include "ragged.cuh"
 
 int mg_sm_count() {

@@ -15,8 +15,9 @@
 // shared memory, whose eight CTAs of 128 KB find room a third at a time. The draw's sums are in 64 bits: with 10^5 entries
 // the running sum's steps are so close that 32-bit sums put the drawn index one off in about one of a hundred draws,
 // where 64-bit sums of 64-bit exponentials do in none.
-// 48 requests of 1 to 8 drafts, 128256 entries, draft probabilities (162 MB, 25 us at 6.55 TB/s): 86 us, of which the rows'
-// states take 32, and the decision and the rest 27 each: a chain of dependent loads, then 64-bit exponentials.
+// 48 requests of 1 to 8 drafts, 128256 entries, draft probabilities (162 MB, 25 us at 6.55 TB/s): 85 us. By
+// themselves the rows' states take 32, the decision 33 and the rest 30 (they overlap in part): the latter two are a chain of
+// dependent loads, then 64-bit exponentials.
 #include "common.cuh"
 
 namespace {

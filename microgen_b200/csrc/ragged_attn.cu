@@ -34,15 +34,16 @@
 //     cycles, two warpgroups sharing an SM's exponentials) and then its own two products (1.0 k); the two row tiles
 //     overlap to 3.2 k cycles, of which the products of both fill two thirds. Tried and slower: the products of each row
 //     tile from a warp of its own (they interleave, and both softmaxes wait for both; a fifth), steps of 64 keys with two
-//     score buffers (a third), reading the scores from tensor memory twice instead of holding 128 of them (up to a tenth). A part
-//     of the exponentials as polynomials, and the rescaling of O behind them, gained nothing;
-//   * 32 requests of 5 tokens over 300 to 4000 cached ones, 60 us, floor 35: the longest CTA's share is 1.2 times the mean,
-//     and the merge adds 5;
+//     score buffers (a third), reading the scores from tensor memory twice instead of holding 128 of them (up to a
+//     tenth). A part of the exponentials as polynomials, and the rescaling of O behind them, gained nothing;
+//   * 32 requests of 5 tokens over 300 to 4000 cached ones, 57 us, floor 35: the longest CTA's share is 1.2 times the mean,
+//     and the merge adds 5 (60 with all loads from one warp, whose 2 KB copies do not start fast enough);
 //   * 24 packed prompts of 18 to 2005 tokens, 14/2 heads of 64, 65 us: the exponentials of whole 128 x 128 tiles, most of
 //     them cut by the diagonal; the products would take 13;
 //   * 16 chunks over up to 3800 cached tokens, bf16, 59 us: two or three short items a CTA, each with an end of its own;
-//     int8, 82: codes to bf16 by one warpgroup (2.0 k cycles a tile) and a softmax of 4.2 k cycles, the scales' products included, in
-//     code that strains the instruction caches (95 while all of it was unrolled, with a row per thread).
+//     int8, 82: codes to bf16 by one warpgroup (2.0 k cycles a tile) and a softmax of 4.2 k cycles, the scales'
+//     products included, in code that strains the instruction caches (95 while all of it was unrolled, with a row per
+//     thread).
 #include <type_traits>
 
 #include "ragged.cuh"
@@ -544,11 +545,14 @@ __global__ void __launch_bounds__(RagCfg<D, Q8>::kThreads, 1)
       if (elect_one()) tc_commit(drained);
       __syncwarp();
       bar_wait(drained, 0, 519);
-    } else if (warp == 9) {
-      // ---------------- K/V loads: K_0, V_0, K_1, V_1, ... ----------------
+    } else if (warp == 9 || warp == 11) {
+      // ---------------- K/V loads: K_0, V_0, K_1, V_1, ..., K by one warp and V by another ----------------
       // bf16: a TMA copy for each block and slab; int8: bulk copies of a block's codes and scales. Lane b < 8 holds the
-      // tile's b-th block id, fetched a tile ahead; one lane starts the copies
-      int i = 0;
+      // tile's b-th block id, fetched a tile ahead; one lane starts the copies. (Where the ring is of odd length, a stage's
+      // loads alternate between the warps. None can take an older release of a stage for the one it waits for: releases
+      // come nearly in the order of the loads, and its own last wait was for a later one than that.)
+      const int kv = warp == 11;
+      int i = kv;  // the next load's place in that order
       const int blk = lane & 7;
       for (int pass = 0; pass < 2; ++pass) {
         walk.start(p, total, pass ? redo : nullptr);
@@ -560,49 +564,46 @@ __global__ void __launch_bounds__(RagCfg<D, Q8>::kThreads, 1)
           const int blocks = (wk.it.kv_len + 15) >> 4;
           int b0 = wk.it.kt0 * 8;
           int32_t id_next = wk.tiles > 0 && b0 + blk < blocks ? table[b0 + blk] : 0;
-          for (int j = 0; j < wk.tiles && ok; ++j, b0 += 8) {
+          for (int j = 0; j < wk.tiles && ok; ++j, b0 += 8, i += 2) {
             const int nb = min(8, blocks - b0);
             const int32_t id = id_next;
             const bool good = id >= 0 && id < p.num_blocks;
             if (blk < nb && !good) mg_record_error(MG_ERR_DEVICE, 511);
             if (b0 + 8 + blk < blocks) id_next = table[b0 + 8 + blk];
-#pragma unroll
-            for (int kv = 0; kv < 2; ++kv, ++i) {
-              if constexpr (Q8) {
-                const int s = i % NC;
-                if (i >= NC) ok = ok && bar_wait(&cempty[s], ((i / NC) - 1) & 1, 512);
-                if (!ok) break;
-                // a block that is not in the pool is read as the pool's first (its error has been recorded)
-                const int row = (good ? id : 0) * p.hkv + wk.head;
-                if (elect_one()) mbar_arrive_expect_tx(&cfull[s], (uint32_t)(nb * 16 * (D + 4)));
+            if constexpr (Q8) {
+              const int s = i % NC;
+              if (i >= NC) ok = ok && bar_wait(&cempty[s], ((i / NC) - 1) & 1, 512);
+              if (!ok) break;
+              // a block that is not in the pool is read as the pool's first (its error has been recorded)
+              const int row = (good ? id : 0) * p.hkv + wk.head;
+              if (elect_one()) mbar_arrive_expect_tx(&cfull[s], (uint32_t)(nb * 16 * (D + 4)));
 #pragma unroll 1
-                for (int y = 0; y < 8; ++y) {
-                  const int64_t r = (int64_t)__shfl_sync(0xffffffffu, row, y) * 16;
-                  if (y < nb && elect_one()) {
-                    bulk_load_smem(smem + C::kCodes + s * C::kCodeBytes + y * 16 * D, (kv ? p.v8 : p.k8) + r * D, 16 * D,
-                                   &cfull[s]);
-                    bulk_load_smem(smem + C::kCodeScales + s * kRows * 4 + y * 64, (kv ? p.vs : p.ks) + r, 64, &cfull[s]);
-                  }
-                  __syncwarp();
+              for (int y = 0; y < 8; ++y) {
+                const int64_t r = (int64_t)__shfl_sync(0xffffffffu, row, y) * 16;
+                if (y < nb && elect_one()) {
+                  bulk_load_smem(smem + C::kCodes + s * C::kCodeBytes + y * 16 * D, (kv ? p.v8 : p.k8) + r * D, 16 * D,
+                                 &cfull[s]);
+                  bulk_load_smem(smem + C::kCodeScales + s * kRows * 4 + y * 64, (kv ? p.vs : p.ks) + r, 64, &cfull[s]);
                 }
-              } else {
-                const int s = i % NS;
-                if (i >= NS) ok = ok && bar_wait(&empty[s], ((i / NS) - 1) & 1, 512);
-                if (!ok) break;
-                // (a block that is not in the pool is read behind its end: as zeros)
-                const int row = (int)(good ? (id * p.hkv + wk.head) * 16 : p.num_blocks * p.hkv * 16);
-                if (elect_one()) mbar_arrive_expect_tx(&full[s], (uint32_t)(nb * 16 * D * 2));
+                __syncwarp();
+              }
+            } else {
+              const int s = i % NS;
+              if (i >= NS) ok = ok && bar_wait(&empty[s], ((i / NS) - 1) & 1, 512);
+              if (!ok) break;
+              // (a block that is not in the pool is read behind its end: as zeros)
+              const int row = (int)(good ? (id * p.hkv + wk.head) * 16 : p.num_blocks * p.hkv * 16);
+              if (elect_one()) mbar_arrive_expect_tx(&full[s], (uint32_t)(nb * 16 * D * 2));
 #pragma unroll
-                for (int y = 0; y < 8; ++y) {
-                  const int r = __shfl_sync(0xffffffffu, row, y);
-                  if (y < nb && elect_one()) {
+              for (int y = 0; y < 8; ++y) {
+                const int r = __shfl_sync(0xffffffffu, row, y);
+                if (y < nb && elect_one()) {
 #pragma unroll
-                    for (int x = 0; x < C::kSlabs; ++x)
-                      tma_load_2d(smem + C::kRing + s * C::kTileBytes + x * C::kSlabBytes + y * 16 * C::kSlab, kv ? &tv : &tk,
-                                  &full[s], x * (C::kSlab / 2), r);
-                  }
-                  __syncwarp();
+                  for (int x = 0; x < C::kSlabs; ++x)
+                    tma_load_2d(smem + C::kRing + s * C::kTileBytes + x * C::kSlabBytes + y * 16 * C::kSlab, kv ? &tv : &tk,
+                                &full[s], x * (C::kSlab / 2), r);
                 }
+                __syncwarp();
               }
             }
           }
@@ -612,10 +613,13 @@ __global__ void __launch_bounds__(RagCfg<D, Q8>::kThreads, 1)
         if (!*redo_any) break;
       }
       // the loads that were started have landed before this CTA's memory goes to another
+      const int all = i - kv;
       if constexpr (Q8) {
-        for (int x = max(0, i - NC); x < i; ++x) bar_wait(&cfull[x % NC], (x / NC) & 1, 513);
+        for (int x = max(0, all - NC); x < all; ++x)
+          if ((x & 1) == kv) bar_wait(&cfull[x % NC], (x / NC) & 1, 513);
       } else {
-        for (int x = max(0, i - NS); x < i; ++x) bar_wait(&full[x % NS], (x / NS) & 1, 513);
+        for (int x = max(0, all - NS); x < all; ++x)
+          if ((x & 1) == kv) bar_wait(&full[x % NS], (x / NS) & 1, 513);
       }
     } else if (warp == 10) {
       // ---------------- Q loads: a row tile's tokens x heads of the group, as soon as the products before are done ------
@@ -648,8 +652,6 @@ __global__ void __launch_bounds__(RagCfg<D, Q8>::kThreads, 1)
       }
       if (c0 > 0) bar_wait(&qfull[0], (c0 - 1) & 1, 525);
       if (c1 > 0) bar_wait(&qfull[1], (c1 - 1) & 1, 525);
-    } else if (!Q8 && warp == 11) {
-      block_barrier();  // (the passes' barrier; this warp has no part in either)
     } else if (Q8 && warp >= 12) {
       // ---------------- int8 codes -> bf16 tiles, swizzled ----------------
       const int t = threadIdx.x - 12 * 32;
@@ -1071,7 +1073,8 @@ __global__ void __launch_bounds__(RagCfg<D, Q8>::kThreads, 1)
           if (it.slot >= 0 && t < valid) p.ws_ml[slot_row] = make_float2(ml, l);
           if (!Q8 && !kAgain && t < valid && odd_sum != 0.f) {
             // Zero times an infinite or NaN value of a masked key may be in there: the piece is done over with a look at V.
-            atomicOr(const_cast<uint32_t*>(redo + min(piece >> 5, kRedoWords - 1)), 1u << (piece < 32 * kRedoWords ? piece & 31 : 31));
+            atomicOr(const_cast<uint32_t*>(redo + min(piece >> 5, kRedoWords - 1)),
+                     1u << (piece < 32 * kRedoWords ? piece & 31 : 31));
             *redo_any = 1;
           }
         }
@@ -1102,7 +1105,7 @@ __global__ void __launch_bounds__(RagCfg<D, Q8>::kThreads, 1)
 // table, states and outputs): so the rows of all items are dealt out evenly over as many warps as the machine holds, and
 // the first batch of outputs is fetched while the states are.
 // Measured (attention and merge): 16 chunks over up to 3800 cached tokens, 71.5 us with a CTA for every item, head and
-// eighth of the rows, 59.6 so; 62 with batches of eight parts, which only a single token over a long cache gains from (1 of 38).
+// eighth of the rows, 59.6 so; 62 with batches of eight parts, which only a single token over a long cache gains from.
 constexpr int kMergeWarps = 8;
 constexpr int kMergeBatch = 4;  // parts in flight
 constexpr int kMergeCtas = 4;   // CTAs that an SM holds
@@ -1123,7 +1126,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32, kMergeCtas) ragged_merge_ker
   const int lane = threadIdx.x & 31;
   const RagMerge* items = reinterpret_cast<const RagMerge*>(p.work + p.merge_off);
   const int n_items = min(reinterpret_cast<const RagHead*>(p.work)->n_merge, p.max_slots / 2);
-  // (all slots together hold fewer than 2^31 values: max_slots * hkv is at most 2 * max(multiprocessors, hkv))
+  // (32-bit indices of a row's 32 vectors: max_slots * hkv is at most 2 * max(multiprocessors, hkv), below 2^18)
   const int step = p.hkv * (2 * kRows);
   int unit = (int)blockIdx.x * kMergeWarps + (threadIdx.x >> 5);  // the warp's next (item, row, head) ...
   int before = 0;                                                 // ... and those of the items passed so far
@@ -1131,7 +1134,8 @@ __global__ void __launch_bounds__(kMergeWarps * 32, kMergeCtas) ragged_merge_ker
     RagMerge mine = {};
     if (i0 + lane < n_items) mine = items[i0 + lane];
     const bool fits = mine.row0 >= 0 && (int64_t)mine.row0 + mine.n_tok <= p.rows && mine.slot0 >= 0 &&
-                      mine.n_tok <= 2 * p.tok_tile && mine.parts > 0 && mine.slot0 + mine.parts <= p.max_slots;  // (else the attention kernel has recorded it)
+                      mine.n_tok <= 2 * p.tok_tile && mine.parts > 0 && mine.slot0 + mine.parts <= p.max_slots;
+    // (where it does not, the attention kernel has recorded it)
     const int units = fits ? mine.n_tok * p.group * p.hkv : 0;
     int upto = units;  // units of the lanes up to this one
 #pragma unroll
@@ -1290,8 +1294,10 @@ extern "C" int mg_ragged_attn(const void* q, int64_t rows, const void* k_pool, c
   cudaStream_t st = mg_stream(stream);
   if (q8) {
     if (d == 32) return launch_ragged<32, true>(a, s, q, k_pool, v_pool, st);
-    return d == 64 ? launch_ragged<64, true>(a, s, q, k_pool, v_pool, st) : launch_ragged<128, true>(a, s, q, k_pool, v_pool, st);
+    if (d == 64) return launch_ragged<64, true>(a, s, q, k_pool, v_pool, st);
+    return launch_ragged<128, true>(a, s, q, k_pool, v_pool, st);
   }
   if (d == 32) return launch_ragged<32, false>(a, s, q, k_pool, v_pool, st);
-  return d == 64 ? launch_ragged<64, false>(a, s, q, k_pool, v_pool, st) : launch_ragged<128, false>(a, s, q, k_pool, v_pool, st);
+  if (d == 64) return launch_ragged<64, false>(a, s, q, k_pool, v_pool, st);
+  return launch_ragged<128, false>(a, s, q, k_pool, v_pool, st);
 }

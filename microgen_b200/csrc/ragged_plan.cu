@@ -38,7 +38,7 @@ struct PlanArgs {
   int32_t *cu, *kv_lens, *positions, *slots, *seq_ids, *held_out, *cursor_out;
   uint8_t* work;
   int64_t n_free, num_blocks, max_rows;
-  int b, max_blocks, hkv, sms;
+  int b, max_blocks;
   RagShape s;
 };
 
@@ -348,8 +348,7 @@ extern "C" int mg_ragged_plan(const int32_t* q_lens, const int32_t* ctx_lens, in
     return MG_ERR_INVALID_ARG;
   PlanArgs a{};
   if (b > kPlanMaxB || max_blocks > (1 << 26) || n_free > 0x7fffffff) return MG_ERR_UNSUPPORTED;
-  a.sms = mg_sm_count();
-  if (!rag_shape(max_rows, b, hq, hkv, d, a.sms, &a.s)) return MG_ERR_UNSUPPORTED;
+  if (!rag_shape(max_rows, b, hq, hkv, d, mg_sm_count(), &a.s)) return MG_ERR_UNSUPPORTED;
   if (work_bytes < (size_t)a.s.total) return MG_ERR_INVALID_ARG;
   a.q_lens = q_lens;
   a.ctx_lens = ctx_lens;
@@ -370,7 +369,6 @@ extern "C" int mg_ragged_plan(const int32_t* q_lens, const int32_t* ctx_lens, in
   a.max_rows = max_rows;
   a.b = b;
   a.max_blocks = max_blocks;
-  a.hkv = hkv;
   const size_t smem = ((size_t)5 * b + 2) * sizeof(int32_t);
   static bool done[64] = {};
   static std::mutex mu;

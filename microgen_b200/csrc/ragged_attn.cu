@@ -403,7 +403,10 @@ __global__ void __launch_bounds__(RagCfg<D, Q8>::kThreads, 1)
   uint64_t* drained = merged + 1;
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(drained + 1);
   volatile int* skip = reinterpret_cast<volatile int*>(tmem_holder + 1);  // [2] the softmax threads did a tile's P V
-  volatile int* odd_v = skip + 2;  // [2] an infinity or NaN was found among V rows that some row may not see
+  // [2] the last piece (its place in the CTA's list, from 1) with an infinity or NaN among V rows that some row may not
+  // see. The warps of a warpgroup enter a piece at times of their own, so a flag that one of them cleared there could wipe
+  // out what another has found already; a finding's own name needs no clearing.
+  volatile int* odd_v = skip + 2;
   volatile uint32_t* redo = reinterpret_cast<volatile uint32_t*>(smem + C::kRedo);  // pieces for a second pass ...
   volatile uint32_t* redo_any = redo + kRedoWords;                                   // ... and whether there are any
   auto block_barrier = [] { asm volatile("bar.sync 1, %0;" ::"n"(C::kThreads) : "memory"); };
@@ -745,7 +748,6 @@ __global__ void __launch_bounds__(RagCfg<D, Q8>::kThreads, 1)
         const int first_pos = it.pos0 + tok0, my_pos = first_pos + my_tok;
         const bool warp_on = (warp & 3) * 32 < valid;
         const int n = w ? wk.n1 : wk.n0;
-        if (kAgain && t == 0) odd_v[w] = 0;
         float mr[kR];     // the maxima in use of the thread's rows, in score units
         uint64_t lr[kR];  // the sums, in two halves
 #pragma unroll
@@ -780,13 +782,13 @@ __global__ void __launch_bounds__(RagCfg<D, Q8>::kThreads, 1)
                 const bool odd = odd_rows<D>(v, max(0, first_pos + 1 - key0), min(r_end, kRows), t);
                 // (any thread's finding is every thread's; once found it holds for the piece's later tiles too)
                 if (lane == 0) {
-                  if (odd) odd_v[w] = 1;
+                  if (odd) odd_v[w] = piece + 1;
                   mbar_arrive(&looked[w]);
                 }
                 ok = bar_wait(&looked[w], looks & 1, 523);
                 ++looks;
                 if (!ok) break;
-                by_hand = odd_v[w] != 0;
+                by_hand = odd_v[w] == piece + 1;
               }
             }
           }

@@ -469,6 +469,39 @@ def test_attention_ignores_what_a_row_may_not_see(kv8):
     assert errors()[0] == 0
 
 
+@pytest.mark.parametrize("hq,hkv,d", [(24, 8, 128), (14, 2, 64), (6, 6, 32)])
+@pytest.mark.parametrize("b,q,ctx", [(40, (10, 40), (0, 0)), (64, (5, 5), (0, 100)), (24, (90, 300), (0, 60))])
+def test_attention_ignores_masked_values_of_many_pieces(hq, hkv, d, b, q, ctx):
+    """An infinity or NaN in a late token's V of nearly every request and K/V head, in a column of its own: a CTA has several
+    such pieces one behind another, and what it found in one must not be taken for, or lost in, the next."""
+    rng = np.random.default_rng(b)
+    c = Case(rng.integers(q[0], q[1] + 1, b), rng.integers(ctx[0], ctx[1] + 1, b), hq, hkv, d, seed=b).fill()
+    clean = c.run().clone()
+    want, mag = c.oracle()  # of the clean values
+    bad_row = torch.zeros_like(want, dtype=torch.bool)
+    same = torch.zeros(want.shape[0], dtype=torch.bool, device="cuda")
+    r = 0
+    for i, (n, x) in enumerate(zip(c.q_lens, c.ctx)):
+        t = int(rng.integers(n // 2 + 1, n))
+        if i % 5 == 4:
+            same[r:r + n] = True
+        else:
+            blk, off = c.tables[i, (x + t) // 16], (x + t) % 16
+            for h in range(hkv):
+                col = (7 * i + 13 * h) % d
+                c.v[blk, h, off, col] = (math.nan, math.inf, -math.inf)[(i + h) % 3]
+                bad_row[r + t:r + n, h * (hq // hkv):(h + 1) * (hq // hkv), col] = True
+        r += n
+    bound = 2.0 ** -7 * 1.05 * mag + 1e-6
+    for _ in range(6):
+        out = c.run()
+        assert torch.equal(out[same], clean[same])
+        got = out.double().view_as(want)
+        assert not torch.isfinite(got[bad_row]).any()
+        assert ((got - want).abs() <= bound)[~bad_row].all()
+    assert errors()[0] == 0
+
+
 def test_attention_matches_the_decode_kernel():
     """Single tokens: the operator gives what paged_decode_attn gives (which rounds q * scale to bf16)."""
     c = Case([1] * 6, [3, 63, 500, 1999, 0, 128], 24, 8, 128, seed=8).fill()

@@ -502,6 +502,50 @@ def test_attention_ignores_masked_values_of_many_pieces(hq, hkv, d, b, q, ctx):
     assert errors()[0] == 0
 
 
+NAN_CASES = [([1], [100]), ([1], [128]), ([1], [300]), ([1], [20000]), ([60], [0]), ([200], [100]), ([40, 1], [9000, 7])]
+
+
+@pytest.mark.parametrize("kv8", [False, True])
+@pytest.mark.parametrize("q,ctx", NAN_CASES)
+def test_attention_gives_nan_for_a_nan_that_a_row_sees(q, ctx, kv8):
+    """A NaN in a query, or in the K of a key: NaN in the rows that meet it and in no others, in every form of an item (one
+    row tile or two, whose keys one warpgroup takes or both, split along the keys or not)."""
+    def check(c, bad):
+        want, mag = c.oracle()
+        got = c.run().double().view_as(want)
+        assert torch.isnan(got[bad]).all()
+        assert ((got - want).abs() <= 2.0 ** -7 * 1.05 * mag + 1e-6)[~bad].all()
+        assert errors()[0] == 0
+
+    c = Case(q, ctx, 24, 8, 128, kv8, seed=1).fill()
+    bad = torch.zeros((sum(q), 24), dtype=torch.bool, device="cuda")
+    for r in {0, q[0] // 2, q[0] - 1}:
+        c.q[r, 5 + r % 7, 7] = math.nan
+        bad[r, 5 + r % 7] = True
+    check(c, bad)
+    c = Case(q, ctx, 24, 8, 128, kv8, seed=2).fill()
+    t = q[0] // 2  # the new token whose K holds it
+    at = (c.tables[0, (ctx[0] + t) // 16], 2, (ctx[0] + t) % 16)
+    if kv8:
+        c.sc["k_scales"][at] = math.nan
+    else:
+        c.k[at][3] = math.nan
+    bad = torch.zeros((sum(q), 24), dtype=torch.bool, device="cuda")
+    bad[t:q[0], 6:9] = True
+    check(c, bad)
+
+
+@pytest.mark.parametrize("q,ctx", NAN_CASES)
+def test_attention_gives_nan_where_every_score_is_minus_infinity(q, ctx):
+    c = Case(q, ctx, 24, 8, 128, seed=3).fill()
+    c.q[:, :3] = 1.0
+    c.k[:, 0] = 1.0
+    c.k[:, 0, :, 3] = -math.inf
+    got = c.run().view(-1, 24, 128)
+    assert torch.isnan(got[:, :3]).all() and torch.isfinite(got[:, 3:]).all()
+    assert errors()[0] == 0
+
+
 def test_attention_matches_the_decode_kernel():
     """Single tokens: the operator gives what paged_decode_attn gives (which rounds q * scale to bf16)."""
     c = Case([1] * 6, [3, 63, 500, 1999, 0, 128], 24, 8, 128, seed=8).fill()

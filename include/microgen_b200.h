@@ -320,7 +320,8 @@ int mg_norm_rope_kv_append(const void* qkv, int qkv_bf16, int64_t ld_qkv, int64_
  * rows: at least the plan's; rows behind the last request are left as they were. out must not overlap q. Keys that a row may not see
  * and pool entries behind a request's last token do not affect it, whatever they hold. workspace: device
  * scratch of mg_ragged_attn_workspace_bytes() bytes, 16-byte aligned, contents irrelevant: calls that overlap on
- * the GPU need separate ones. Results do not depend on timing. A plan for other sizes (site 510) or a block id
+ * the GPU need separate ones. Results do not depend on timing. A plan for other sizes
+ * (max_rows, b, hq, hkv or max_blocks differ, or rows is less than the plan's; site 510) or a block id
  * outside the pool (site 511) is recorded; nothing outside the arrays is read. */
 int mg_ragged_attn_workspace_bytes(int64_t max_rows, int b, int hq, int hkv, int d, size_t* bytes);
 int mg_ragged_attn(const void* q, int64_t rows, const void* k_pool, const void* v_pool, const float* k_scales,

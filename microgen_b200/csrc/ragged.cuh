@@ -27,10 +27,15 @@ struct RagShape {
   int64_t list_off, merge_off, total; // byte offsets in the plan's work area
 };
 
-// The first words of the work area.
-struct RagHead {
-  int32_t n_list, n_merge, rows, pad;
+// The first words of the work area. The list's places and items follow from the sizes that the plan was made for, so it
+// leaves them here, and the attention runs no list that was made for others.
+struct __align__(16) RagHead {
+  int32_t n_list, n_merge, rows, max_blocks;
+  int32_t max_rows, b, hq, hkv;
 };
+__device__ __forceinline__ bool rag_made_for(const RagHead& h, int64_t max_rows, int b, int hq, int hkv, int max_blocks) {
+  return h.max_rows == max_rows && h.b == b && h.hq == hq && h.hkv == hkv && h.max_blocks == max_blocks;
+}
 
 // Splitting rule (see ragged_plan.cu): no list entry is longer than the work of one of `sms` equal shares, so an
 // item of n tiles gives ceil(n / share) entries and all of them together at most max_items + sms / hkv.

@@ -239,7 +239,7 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
 }
 
 struct RagArgs {
-  int64_t rows, num_blocks;
+  int64_t rows, max_rows, num_blocks;
   const int32_t* tables;
   int max_blocks, b, hq, hkv, group, tok_tile, max_slots;
   float scale_log2;
@@ -295,7 +295,7 @@ struct RagWalk {
     it = rag_item(p, index);
   }
 };
-// The work of an item; one that does not fit this call's arrays (a plan for other sizes) has no tiles.
+// The work of an item; one that does not fit this call's arrays (fewer rows than the plan has) has no tiles.
 __device__ __forceinline__ RagWork rag_work(const RagArgs& p, const RagItem& it, int index) {
   RagWork w;
   w.it = it;
@@ -448,7 +448,10 @@ __global__ void __launch_bounds__(RagCfg<D, Q8>::kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = 0;  // the CTA holds all of tensor memory
   griddep_wait();
-  const int total = reinterpret_cast<const RagHead*>(p.work)->n_list * p.hkv;
+  const RagHead head = *reinterpret_cast<const RagHead*>(p.work);
+  const bool planned = rag_made_for(head, p.max_rows, p.b, p.hq, p.hkv, p.max_blocks);
+  if (!planned && blockIdx.x == 0 && threadIdx.x == 0) mg_record_error(MG_ERR_DEVICE, 510);
+  const int total = planned ? head.n_list * p.hkv : 0;
 
   if (warp >= 8) {
     regs_dec<C::kOtherRegs>();
@@ -1129,7 +1132,8 @@ __global__ void __launch_bounds__(kMergeWarps * 32, kMergeCtas) ragged_merge_ker
   griddep_launch();  // (after the wait: launched before it, a next attention costs 4 of 65 us where nothing is split)
   const int lane = threadIdx.x & 31;
   const RagMerge* items = reinterpret_cast<const RagMerge*>(p.work + p.merge_off);
-  const int n_items = min(reinterpret_cast<const RagHead*>(p.work)->n_merge, p.max_slots / 2);
+  const RagHead head = *reinterpret_cast<const RagHead*>(p.work);
+  const int n_items = rag_made_for(head, p.max_rows, p.b, p.hq, p.hkv, p.max_blocks) ? head.n_merge : 0;
   // (32-bit indices of a row's 32 vectors: max_slots * hkv is at most 2 * max(multiprocessors, hkv), below 2^18)
   const int step = p.hkv * (2 * kRows);
   int unit = (int)blockIdx.x * kMergeWarps + (threadIdx.x >> 5);  // the warp's next (item, row, head) ...
@@ -1273,6 +1277,7 @@ extern "C" int mg_ragged_attn(const void* q, int64_t rows, const void* k_pool, c
   if (mg_overlap(q, rows * hq * d * 2, out, rows * hq * d * 2)) return MG_ERR_INVALID_ARG;
   RagArgs a{};
   a.rows = rows;
+  a.max_rows = max_rows;
   a.num_blocks = num_blocks;
   a.tables = block_tables;
   a.max_blocks = max_blocks;

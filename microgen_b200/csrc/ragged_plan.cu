@@ -38,9 +38,22 @@ struct PlanArgs {
   int32_t *cu, *kv_lens, *positions, *slots, *seq_ids, *held_out, *cursor_out;
   uint8_t* work;
   int64_t n_free, num_blocks, max_rows;
-  int b, max_blocks;
+  int b, max_blocks, hq, hkv;
   RagShape s;
 };
+
+__device__ __forceinline__ void write_head(const PlanArgs& p, int64_t n_list, int64_t n_merge, int64_t rows) {
+  RagHead h;
+  h.n_list = (int32_t)n_list;
+  h.n_merge = (int32_t)n_merge;
+  h.rows = (int32_t)rows;
+  h.max_blocks = p.max_blocks;
+  h.max_rows = (int32_t)p.max_rows;
+  h.b = p.b;
+  h.hq = p.hq;
+  h.hkv = p.hkv;
+  *reinterpret_cast<RagHead*>(p.work) = h;
+}
 
 // Exclusive prefixes of N values per thread over the CTA's kT threads, in one round of barriers; total gets the sums.
 // red: N * 33 words of shared memory, free for reuse after the next barrier.
@@ -179,8 +192,7 @@ __global__ void __launch_bounds__(kT) plan_kernel(const PlanArgs p) {
     }
     if (g == 0) {
       *p.cursor_out = cursor;
-      RagHead* h = reinterpret_cast<RagHead*>(p.work);
-      h->n_list = h->n_merge = h->rows = 0;
+      write_head(p, 0, 0, 0);
     }
     return;
   }
@@ -292,12 +304,7 @@ __global__ void __launch_bounds__(kT) plan_kernel(const PlanArgs p) {
       }
       if (parts > 1) slot0 += parts;
     }
-    if (t == 0) {
-      RagHead* h = reinterpret_cast<RagHead*>(p.work);
-      h->n_list = (int32_t)entries;
-      h->n_merge = (int32_t)n_merge;
-      h->rows = (int32_t)n_rows;
-    }
+    if (t == 0) write_head(p, entries, n_merge, n_rows);
     return;
   }
   const int64_t g = (int64_t)(rank - 1) * kT + t, step = (int64_t)(kPlanCtas - 1) * kT;
@@ -369,6 +376,8 @@ extern "C" int mg_ragged_plan(const int32_t* q_lens, const int32_t* ctx_lens, in
   a.max_rows = max_rows;
   a.b = b;
   a.max_blocks = max_blocks;
+  a.hq = hq;
+  a.hkv = hkv;
   const size_t smem = ((size_t)5 * b + 2) * sizeof(int32_t);
   static bool done[64] = {};
   static std::mutex mu;

@@ -634,6 +634,39 @@ def test_attention_records_a_plan_for_more_rows():
     assert errors() == (5, 510)
 
 
+@pytest.mark.parametrize("other", [dict(max_rows=700), dict(b=3), dict(hq=16, hkv=16), dict(hq=48), dict(max_blocks=700)])
+def test_attention_records_a_plan_for_other_sizes(other):
+    """A work area that was planned for other sizes has its list elsewhere: it is recorded and nothing of it is run, neither
+    by the attention nor by the merge of split items."""
+    from microgen_b200 import _lib
+    c = Case([1, 40], [9000, 500], 24, 8, 64, seed=1).fill()
+    assert work_list(c.plan)[1].shape[0] > 0
+    p = c.plan
+    a = dict(max_rows=p.max_rows, b=p.b, hq=p.hq, hkv=p.hkv, max_blocks=p.max_blocks)
+    a.update(other)
+    q = torch.zeros((41, a["hq"], 64), dtype=torch.bfloat16, device="cuda")
+    out = torch.full((41, a["hq"] * 64), 2.0, dtype=torch.bfloat16, device="cuda")
+    pool = torch.zeros((c.blocks, a["hkv"], 16, 64), dtype=torch.bfloat16, device="cuda")
+    tables = torch.zeros((a["b"], a["max_blocks"]), dtype=torch.int32, device="cuda")
+    ws = K().RaggedPlan(a["b"], a["max_rows"], a["max_blocks"], a["hq"], a["hkv"], 64, "cuda").workspace
+    _lib.call("mg_ragged_attn", q.data_ptr(), 41, pool.data_ptr(), pool.data_ptr(), None, None, c.blocks, tables.data_ptr(),
+              a["max_blocks"], a["b"], a["max_rows"], a["hq"], a["hkv"], 64, 0.125, p.work.data_ptr(), out.data_ptr(),
+              ws.data_ptr(), ws.numel(), torch.cuda.current_stream().cuda_stream)
+    assert errors() == (5, 510)
+    assert (out == 2).all()
+    check_attn(c, c.run())
+
+
+def test_an_empty_plan_gives_the_attention_nothing_to_do():
+    c = Case([4, 9], [3, 100], 14, 2, 64)
+    c.q_lens[0] = 100  # one length alone is more than the plan's rows
+    c.fill()
+    assert errors() == (5, 500)
+    out = torch.full((13, 14 * 64), 2.0, dtype=torch.bfloat16, device="cuda")
+    c.run(out=out)
+    assert errors()[0] == 0 and (out == 2).all()
+
+
 # ---------------------------------------------------------------- verification
 def verify_oracle(logits, tokens, cu, u, probs, temps):
     lg = logits.double().cpu().numpy()

@@ -354,11 +354,11 @@ __global__ void __launch_bounds__(kStatThreads) verify_decide_kernel(const Verif
   }
   const int n = (int)(r1 - r0 - 1);
   const float T = p.temps ? p.temps[req] : 1.f;
-  const bool greedy = !(T > 0.f);
+  const bool greedy = !(T > 0.f), bad_t = !(T >= 0.f);
   const float c = greedy ? 0.f : 1.4426950408889634f / T;
   if (t == 0) {
     s_stop = n;
-    s_bad = T < 0.f || T != T ? 602 : 0;
+    s_bad = 0;
   }
   __syncthreads();
   // one warp per row: the row's state from its chunks, then the test of its draft
@@ -398,12 +398,12 @@ __global__ void __launch_bounds__(kStatThreads) verify_decide_kernel(const Verif
     }
   }
   __syncthreads();
-  const int bad = s_bad;
-  const bool answered = greedy || bad == 602 || bad == 604;
+  const int bad = bad_t ? 602 : s_bad;  // (without a temperature there is no answer, whatever else is wrong)
+  const bool answered = greedy || bad == 604;
   if (seg == 0 && t == 0) {
     if (bad) mg_record_error(MG_ERR_DEVICE, bad);
-    p.accepted[req] = bad == 602 ? 0 : stop;
-    if (answered) p.next[req] = bad == 602 || bad == 604 ? -1 : s_next;
+    p.accepted[req] = bad_t ? 0 : stop;
+    if (answered) p.next[req] = bad_t || bad == 604 ? -1 : s_next;
     out->stop = stop;
     out->max = s_max;
     out->draw = answered ? 0 : (stop < n ? 2 : 1);

@@ -865,6 +865,19 @@ def test_verify_records_what_it_cannot_answer(what, site):
     assert (acc[ok].item(), nxt[ok].item()) == (want[0][ok], want[1][ok])
 
 
+@pytest.mark.parametrize("t", [-1.0, math.nan])
+def test_verify_bad_temperature_beside_a_bad_draft(t):
+    """Two things wrong with one request: without a temperature there is no answer, whatever its drafts are."""
+    logits, tokens, cu, u, _ = verify_case([2, 2], 100, False, 3)
+    tokens = tokens.copy()
+    tokens[1] = 100
+    temps = torch.tensor([t, 1.0], device="cuda")
+    acc, nxt = K().verify_drafts(logits, i32(tokens), i32(cu), u, temperatures=temps)
+    assert errors() == (5, 602)
+    want = verify_oracle(logits, tokens.clip(0, 99), cu, u.cpu().numpy(), None, None)
+    assert (acc.tolist(), nxt.tolist()) == ([0, want[0][1]], [-1, want[1][1]])
+
+
 def test_verify_invalid_draft_behind_the_stop():
     """A drafted token outside the vocabulary behind the place where the request stops is recorded, and changes nothing:
     the token that was turned down is still not drawn again."""

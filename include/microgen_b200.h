@@ -237,7 +237,8 @@ int mg_paged_decode_attn(const float* q, const void* k_pool, const void* v_pool,
  * Pools int8 [num_blocks, hkv, 16, d] and one fp32 scale per (block, kv head, token) vector in
  * k_scales / v_scales [num_blocks, hkv, 16] (16-byte aligned). mg_rope_kv_append_kv8: as
  * mg_rope_kv_append, then each K and V vector of d values x is stored as s = max(max|x| / 127, 1e-8),
- * code = clamp(round_half_even(x / s), -128, 127) — the reference's _quantize_tensor over head_dim.
+ * code = clamp(round_half_even(x / s), -128, 127) — the reference's _quantize_tensor over head_dim. The maximum
+ * passes over a NaN, which is stored as code -128.
  * mg_paged_decode_attn_kv8: as mg_paged_decode_attn over those pools, with K and V the codes times their
  * scales (the codes enter the tensor cores exactly; the scales multiply the scores and the probabilities).
  * Workspace bytes as mg_paged_attn_workspace_bytes. The step's own token is read back quantized, where the
@@ -305,7 +306,8 @@ int mg_ragged_plan(const int32_t* q_lens, const int32_t* ctx_lens, int b, int64_
  * q_weight / k_weight fp32 [d] (NULL = no norm): y = x * rsqrt(mean(x^2) + eps) * weight over each head; cos_sin as
  * for mg_rope_kv_append (NULL = no rotation); q_out [rows, hq, d] in bf16 (q_bf16 != 0) or fp32. K and V go to
  * slots[i] of the pools: bf16, or with k_scales / v_scales int8 codes and scales as mg_rope_kv_append_kv8 stores
- * them. A row with a negative slot is padding: nothing is written for it; the other slots of a call are distinct.
+ * them, except that a vector with an infinity or NaN reads back as NaN throughout. A row with a negative slot is
+ * padding: nothing is written for it; the other slots of a call are distinct.
  * A position outside the table (site 210) or a slot outside the pool (site 211) is recorded and not written.
  * q_out must not overlap qkv. d in {32, 64, 128}. */
 int mg_norm_rope_kv_append(const void* qkv, int qkv_bf16, int64_t ld_qkv, int64_t rows, const int32_t* positions,

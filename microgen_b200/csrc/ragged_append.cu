@@ -3,7 +3,8 @@
 //   y = x * rsqrt(mean(x^2) + eps) * w          (q and k heads, where a weight is given)
 //   z_j = y_j cos_j - y_{j+d/2} sin_j,  z_{j+d/2} = y_{j+d/2} cos_j + y_j sin_j   (q and k heads, where a table is)
 // q goes out in bf16 or fp32, K and V into their slot of the pools in bf16, or as int8 codes with one scale per
-// vector: s = max(max|z| / 127, 1e-8), code = clamp(round_half_even(z / s), -128, 127).
+// vector: s = max(max|z| / 127, 1e-8), code = clamp(round_half_even(z / s), -128, 127). An infinity or NaN in z makes s one:
+// the whole vector then reads back as NaN.
 //
 // Bound by memory: every value is read once and written once. d / 8 lanes hold a head, each with four adjacent
 // values of the first half and their four rotation partners of the second, so that loads are 16 bytes, the
@@ -45,13 +46,21 @@ __device__ __forceinline__ void store4_bf16(__nv_bfloat16* p, const float4& a) {
   *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16x2(a.x, a.y), pack_bf16x2(a.z, a.w));
 }
 
+// The larger of two, or NaN where either is one.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+// Codes of four values. A quotient that is NaN has code 0: beside the scale that it has then (NaN, or infinite), any value of
+// the vector reads back as NaN.
 __device__ __forceinline__ uint32_t code4(const float4& a, float s) {
   const float v[4] = {a.x, a.y, a.z, a.w};
   uint32_t w = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float c = fminf(fmaxf(rintf(__fdiv_rn(v[i], s)), -128.f), 127.f);
-    w |= ((uint32_t)(int)c & 0xffu) << (8 * i);
+    const int c = min(max(__float2int_rn(__fdiv_rn(v[i], s)), -128), 127);
+    w |= ((uint32_t)c & 0xffu) << (8 * i);
   }
   return w;
 }
@@ -117,10 +126,10 @@ __global__ void __launch_bounds__(kAppThreads) norm_rope_append_kernel(const App
     }
     float mx = 0.f;
     if constexpr (Q8) {
-      mx = fmaxf(fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))),
-                 fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w))));
+      mx = max_nan(max_nan(max_nan(fabsf(x.x), fabsf(x.y)), max_nan(fabsf(x.z), fabsf(x.w))),
+                   max_nan(max_nan(fabsf(y.x), fabsf(y.y)), max_nan(fabsf(y.z), fabsf(y.w))));
 #pragma unroll
-      for (int o = L / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      for (int o = L / 2; o > 0; o >>= 1) mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, o));
     }
     if (!ok) continue;
     if (is_q) {
@@ -144,7 +153,7 @@ __global__ void __launch_bounds__(kAppThreads) norm_rope_append_kernel(const App
     const int kh = hd[k] - p.hq - (is_k ? 0 : p.hkv);
     const int64_t at = (blk * p.hkv + kh) * 16 + (slot[k] & 15);
     if constexpr (Q8) {
-      const float s = fmaxf(__fdiv_rn(mx, 127.f), 1e-8f);
+      const float s = max_nan(__fdiv_rn(mx, 127.f), 1e-8f);
       uint8_t* dst = static_cast<uint8_t*>(is_k ? p.k_pool : p.v_pool) + at * D + j;
       *reinterpret_cast<uint32_t*>(dst) = code4(x, s);
       *reinterpret_cast<uint32_t*>(dst + D / 2) = code4(y, s);

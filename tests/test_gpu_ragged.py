@@ -316,6 +316,33 @@ def test_append_records_bad_positions_and_slots():
     assert errors() == (5, 211)
 
 
+@pytest.mark.parametrize("hq,hkv,d", [(14, 2, 64), (6, 6, 32), (3, 1, 128)])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_append_int8_keeps_what_is_not_a_number(hq, hkv, d, bad):
+    """A vector with an infinity or NaN reads back as NaN; the vectors beside it are stored as without it."""
+    rng = np.random.default_rng(d)
+    rows = 9
+    x = torch.from_numpy(rng.standard_normal((rows, (hq + 2 * hkv) * d)).astype(np.float32)).cuda()
+    slots = i32(rng.permutation(32)[:rows])
+
+    def run(qkv):
+        kp, vp = (torch.zeros((2, hkv, 16, d), dtype=torch.int8, device="cuda") for _ in range(2))
+        ks, vs = (torch.zeros((2, hkv, 16), device="cuda") for _ in range(2))
+        K().norm_rope_kv_append(qkv, None, None, slots, hq, hkv, d, kp, vp, k_scales=ks, v_scales=vs)
+        at = lambda p, s: (p.float() * s[..., None]).transpose(1, 2).reshape(32, hkv, d)[slots.long()]
+        return torch.cat([at(kp, ks), at(vp, vs)], 1)  # [rows, 2 hkv, d]: K's vectors, then V's
+
+    clean = run(x)
+    hit = torch.zeros((rows, 2 * hkv), dtype=torch.bool, device="cuda")
+    heads = x.view(rows, -1, d)
+    for r, h, c in ((1, 0, 0), (1, 2 * hkv - 1, d - 1), (4, hkv, d // 2), (8, hkv - 1, 5)):
+        heads[r, hq + h, c] = bad
+        hit[r, h] = True
+    got = run(x)
+    assert torch.isnan(got[hit]).all() and torch.equal(got[~hit], clean[~hit])
+    assert errors()[0] == 0
+
+
 # ---------------------------------------------------------------- attention
 class Case:
     def __init__(self, q, ctx, hq, hkv, d, kv8=False, seed=0, pad=0, spread=1.0):

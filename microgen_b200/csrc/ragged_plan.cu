@@ -182,7 +182,8 @@ __global__ void __launch_bounds__(kT) plan_kernel(const PlanArgs p) {
       if (i < p.b) {
         p.kv_lens[i] = 0;
         if (p.held && p.held_out != p.held) p.held_out[i] = p.held[i];
-        if (!p.held) p.held_out[i] = 0;
+        // (not held[i]: that is what the step would have needed where there is no free list)
+        if (!p.held) p.held_out[i] = ctx[i] > 0 ? (int32_t)(((int64_t)ctx[i] + 15) >> 4) : 0;
       }
     }
     for (int64_t r = g; r < p.max_rows; r += step) {

@@ -190,6 +190,25 @@ def test_plan_refuses_impossible_lengths(fault, site):
     assert plan.work[:8].tolist() == [0] * 8  # no work for the attention: it leaves its output alone
 
 
+@pytest.mark.parametrize("free", [False, True])
+def test_plan_refused_without_held_counts_leaves_those_of_the_context(free):
+    """``n_blocks`` not given stands for the blocks of ctx: that is what a refused step leaves, and a step after it that takes
+    the plan's own counts goes on from there."""
+    width, ctx = 6, [33, 0, 16, 1]
+    plan = K().RaggedPlan(4, 8, width, 8, 2, 64, "cuda")
+    tables = i32(np.arange(4 * width).reshape(4, width))
+    kw = dict(free_blocks=i32(np.arange(24, 40))) if free else {}
+    K().ragged_plan(plan, i32([3, 4, 5, 6]), i32(ctx), tables, 40, **kw)
+    assert errors() == (5, 503)
+    assert plan.n_blocks.tolist() == [3, 0, 1, 1]
+    K().ragged_plan(plan, i32([9, -1, 0, 0]), i32([33, 0, -7, 1]), tables, 40, **kw)
+    assert errors() == (5, 500)
+    assert plan.n_blocks.tolist() == [3, 0, 0, 1]
+    if free:
+        K().ragged_plan(plan, i32([3, 0, 0, 0]), i32([33, 0, 0, 1]), tables, 40, n_blocks=plan.n_blocks, **kw)
+        assert errors()[0] == 0 and plan.n_blocks.tolist() == [3, 0, 0, 1]
+
+
 def test_plan_records_bad_block_ids():
     plan = K().RaggedPlan(2, 4, 2, 8, 2, 64, "cuda")
     K().ragged_plan(plan, i32([2, 2]), i32([0, 15]), i32([[5, 0], [1, 9]]), 9)

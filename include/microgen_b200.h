@@ -308,7 +308,8 @@ int mg_ragged_plan(const int32_t* q_lens, const int32_t* ctx_lens, int b, int64_
  * slots[i] of the pools: bf16, or with k_scales / v_scales int8 codes and scales as mg_rope_kv_append_kv8 stores
  * them, except that a vector with an infinity or NaN reads back as NaN throughout. A row with a negative slot is
  * padding: nothing is written for it; the other slots of a call are distinct.
- * A position outside the table (site 210) or a slot outside the pool (site 211) is recorded and not written.
+ * A position outside the table (site 210) is recorded, and nothing of its row is written; a slot outside the pool
+ * (site 211) is recorded, and the row's K and V are not written.
  * q_out must not overlap qkv. d in {32, 64, 128}. */
 int mg_norm_rope_kv_append(const void* qkv, int qkv_bf16, int64_t ld_qkv, int64_t rows, const int32_t* positions,
                            const float* cos_sin, int max_pos, const int32_t* slots, const float* q_weight,

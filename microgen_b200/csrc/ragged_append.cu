@@ -112,11 +112,11 @@ __global__ void __launch_bounds__(kAppThreads) norm_rope_append_kernel(const App
       }
     }
     bool ok = on;
-    if (p.cos_sin && on && (is_q || is_k)) {
-      if (pos[k] < 0 || pos[k] >= p.max_pos) {
+    if (p.cos_sin && on) {
+      if (pos[k] < 0 || pos[k] >= p.max_pos) {  // (nothing of such a row is written, V neither)
         if (l == 0) mg_record_error(MG_ERR_DEVICE, 210);
         ok = false;
-      } else {
+      } else if (is_q || is_k) {
         const float* cs = p.cos_sin + (int64_t)pos[k] * D;
         const float4 c = __ldg(reinterpret_cast<const float4*>(cs + j)), s = __ldg(reinterpret_cast<const float4*>(cs + D / 2 + j));
         const float4 u = x, v = y;

@@ -335,6 +335,22 @@ def test_append_records_bad_positions_and_slots():
     assert errors() == (5, 211)
 
 
+@pytest.mark.parametrize("kv8", [False, True])
+@pytest.mark.parametrize("pos", [-1, 5, 2 ** 31 - 1])
+def test_append_writes_nothing_of_a_row_outside_the_table(pos, kv8):
+    hq, hkv, d = 2, 1, 64
+    dt = torch.int8 if kv8 else torch.bfloat16
+    kp, vp = (torch.full((2, hkv, 16, d), 7, dtype=dt, device="cuda") for _ in range(2))
+    sc = dict(k_scales=torch.full((2, hkv, 16), 7.0, device="cuda"), v_scales=torch.full((2, hkv, 16), 7.0, device="cuda")) if kv8 else {}
+    q = torch.full((3, hq, d), 7.0, dtype=torch.bfloat16, device="cuda")
+    K().norm_rope_kv_append(torch.ones((3, 4 * d), device="cuda"), i32([1, pos, 4]), torch.ones((5, d), device="cuda"), i32([3, 4, 5]),
+                            hq, hkv, d, kp, vp, q_out=q, **sc)
+    assert errors() == (5, 210)
+    for t in (kp[0, 0], vp[0, 0], *(s[0, 0] for s in sc.values())):
+        assert (t[4] == 7).all() and (t[3] != 7).any() and (t[5] != 7).any()
+    assert (q[1] == 7).all() and (q[0] != 7).all() and (q[2] != 7).all()
+
+
 @pytest.mark.parametrize("hq,hkv,d", [(14, 2, 64), (6, 6, 32), (3, 1, 128)])
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
 def test_append_int8_keeps_what_is_not_a_number(hq, hkv, d, bad):

@@ -342,7 +342,8 @@ int mg_ragged_attn(const void* q, int64_t rows, const void* k_pool, const void* 
  * (NaN counting as the maximum), which is also the next token. accepted int32 [b], next int32 [b]. A request
  * without rows gets (0, -1). Recorded as MG_ERR_DEVICE: cu_rows outside the rows (601) or T < 0 (602), a row without
  * a softmax (a NaN or +inf logit, or all -inf; 604): next = -1; a drafted token outside the vocabulary (603), which
- * counts as rejected. workspace: mg_verify_workspace_bytes(), 16-byte aligned. */
+ * counts as rejected. accepted and next overlap neither each other nor an input. workspace:
+ * mg_verify_workspace_bytes(), 16-byte aligned. */
 int mg_verify_workspace_bytes(int64_t rows, int64_t vocab, int b, size_t* bytes);
 int mg_verify_drafts(const float* logits, int64_t ld, int64_t rows, int64_t vocab, const int32_t* tokens,
                      const int32_t* cu_rows, int b, const float* draft_probs, int64_t ld_probs,

@@ -506,6 +506,17 @@ extern "C" int mg_verify_drafts(const float* logits, int64_t ld, int64_t rows, i
       workspace_bytes < need || (need && !workspace) || (reinterpret_cast<uintptr_t>(workspace) & 15))
     return MG_ERR_INVALID_ARG;
   if (b == 0) return MG_OK;
+  // (a request is answered while others are still at work on the inputs and on the workspace)
+  const struct { const void* at; int64_t bytes; } held[] = {
+      {logits, rows > 0 ? ((rows - 1) * ld + vocab) * 4 : 0}, {tokens, rows * 4}, {cu_rows, ((int64_t)b + 1) * 4},
+      {draft_probs, draft_probs && rows > 0 ? ((rows - 1) * ld_probs + vocab) * 4 : 0}, {uniforms, rows * 4},
+      {temperatures, temperatures ? (int64_t)b * 4 : 0}, {workspace, (int64_t)need}};
+  const int64_t out_bytes = (int64_t)b * 4;
+  if (mg_overlap(accepted, out_bytes, next, out_bytes)) return MG_ERR_INVALID_ARG;
+  for (const auto& h : held) {
+    if (h.bytes > 0 && (mg_overlap(accepted, out_bytes, h.at, h.bytes) || mg_overlap(next, out_bytes, h.at, h.bytes)))
+      return MG_ERR_INVALID_ARG;
+  }
   VerifyArgs a{};
   a.logits = logits;
   a.ld = ld;

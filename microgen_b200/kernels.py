@@ -423,7 +423,8 @@ def verify_drafts(logits, tokens, cu_rows, uniforms, draft_probs=None, temperatu
     [b+1]), its last accepted token's and then one per draft; ``tokens`` int32 [rows] are the tokens that were fed
     (so row r asks about tokens[r+1]); ``uniforms`` fp32 [rows] in [0, 1); ``draft_probs`` fp32 [rows, vocab], the
     draft's distribution at each asking row (None: the drafts were certain); ``temperatures`` fp32 [b] (None: 1; 0:
-    greedy). Returns (accepted int32 [b], next token int32 [b]); see ``mg_verify_drafts`` for the rule."""
+    greedy). Returns (accepted int32 [b], next token int32 [b]), which as given buffers overlap neither each other nor an
+    input; see ``mg_verify_drafts`` for the rule."""
     if logits.dim() != 2 or logits.stride(1) != 1 or logits.shape[1] < 1:
         raise ValueError("logits must be [rows, vocab] with unit inner stride")
     rows, vocab = logits.shape

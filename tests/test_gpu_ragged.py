@@ -963,6 +963,19 @@ def test_verify_at_the_edges_of_the_uniform_numbers():
     assert errors()[0] == 0
 
 
+def test_verify_refuses_outputs_over_inputs():
+    logits, tokens, cu, u, _ = verify_case([2, 2], 100, False, 3)
+    tokens, cu = i32(tokens), i32(cu)
+    buf = i32(np.zeros(5))
+    from microgen_b200 import _lib
+    for kw in (dict(next_tokens=tokens[:2]), dict(accepted=tokens[4:]), dict(next_tokens=cu[1:]), dict(accepted=buf[:2], next_tokens=buf[1:3])):
+        with pytest.raises(_lib.MGError):
+            K().verify_drafts(logits, tokens, cu, u, **kw)
+    K().verify_drafts(logits, tokens, cu, u, accepted=buf[:2], next_tokens=buf[2:4])  # side by side is well
+    want = verify_oracle(logits, tokens.cpu().numpy(), cu.cpu().numpy(), u.cpu().numpy(), None, None)
+    assert buf.tolist() == want[0] + want[1] + [0] and errors()[0] == 0
+
+
 def test_verify_greedy_takes_nan_as_the_maximum():
     logits, tokens, cu, u, _ = verify_case([1], 300, False, 4)
     logits[0, 77] = math.nan

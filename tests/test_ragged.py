@@ -113,6 +113,26 @@ def test_verify_refusals(lib):
     assert _verify(lib, b=70000, nbytes=1 << 40) == UNSUP
 
 
+def test_verify_outputs_over_inputs_are_refused(lib):
+    """Requests are answered while others still read: no output may lie on an input, on the workspace or on the other output.
+    (Only refusals are called here: the addresses are made up.)"""
+    at = {n: 0x10000000 * (i + 1) for i, n in enumerate(("logits", "tokens", "cu", "probs", "u", "temps", "acc", "next", "ws"))}
+    rows, vocab, b = 5, 100, 3
+
+    def call(**kw):
+        a = {k: ctypes.c_void_p(v) for k, v in {**at, **kw}.items()}
+        return lib.mg_verify_drafts(a["logits"], vocab, rows, vocab, a["tokens"], a["cu"], b, a["probs"], vocab, a["u"], a["temps"],
+                                    a["acc"], a["next"], a["ws"], 1 << 20, None)
+
+    size = dict(logits=rows * vocab * 4, tokens=rows * 4, cu=(b + 1) * 4, probs=rows * vocab * 4, u=rows * 4, temps=b * 4, ws=512)
+    for name, n in size.items():
+        for out in ("acc", "next"):
+            assert call(**{out: at[name]}) == BAD
+            assert call(**{out: at[name] + n - 4}) == BAD
+            assert call(**{out: at[name] - b * 4 + 4}) == BAD
+    assert call(acc=at["next"]) == BAD and call(next=at["acc"] + 8) == BAD
+
+
 def test_wrappers_refuse_host_tensors():
     i = torch.zeros(2, dtype=torch.int32)
     x = torch.zeros(2, 12 * 64)

@@ -54,6 +54,11 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// log2(e) / T, finite for the smallest T too: the maximum's own exponent is 0 times it.
+__device__ __forceinline__ float exponent_factor(float T) {
+  return T > 0.f ? fminf(1.4426950408889634f / T, 3.402823466e38f) : 0.f;
+}
+
 // (m, s) <- merge of two (max, sum of exp2((x - max) * c)) states.
 __device__ __forceinline__ void merge_ms(float& m, float& s, float om, float os, float c) {
   const float nm = fmaxf(m, om);
@@ -92,7 +97,7 @@ __global__ void __launch_bounds__(kStatThreads) verify_stats_kernel(const Verify
   const int req = seen - 1;
   if (req < 0 || req >= p.b) return;  // a row behind the last request
   const float T = p.temps ? p.temps[req] : 1.f;
-  const float c = T > 0.f ? 1.4426950408889634f / T : 0.f;
+  const float c = exponent_factor(T);
   float m = -INFINITY, s = 0.f, best = -INFINITY;
   int32_t bi = 0x7fffffff;
   if (T > 0.f) {
@@ -355,7 +360,7 @@ __global__ void __launch_bounds__(kStatThreads) verify_decide_kernel(const Verif
   const int n = (int)(r1 - r0 - 1);
   const float T = p.temps ? p.temps[req] : 1.f;
   const bool greedy = !(T > 0.f), bad_t = !(T >= 0.f);
-  const float c = greedy ? 0.f : 1.4426950408889634f / T;
+  const float c = exponent_factor(T);
   if (t == 0) {
     s_stop = n;
     s_bad = 0;

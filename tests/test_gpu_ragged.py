@@ -976,6 +976,19 @@ def test_verify_refuses_outputs_over_inputs():
     assert buf.tolist() == want[0] + want[1] + [0] and errors()[0] == 0
 
 
+@pytest.mark.parametrize("probs", [False, True])
+@pytest.mark.parametrize("t", [1e-44, 1e-40, 4e-39, 1e-37, 1e-30, 1e30])
+def test_verify_extreme_temperatures(t, probs):
+    """Any T > 0 is a temperature, the smallest numbers that fp32 has among them, where the softmax is the maximum's alone; and
+    large ones, where all tokens are nearly alike."""
+    logits, tokens, cu, u, q = verify_case([3, 0, 2, 5], 20000, probs, 8)
+    temps = np.full(4, t, np.float32)
+    got = K().verify_drafts(logits, i32(tokens), i32(cu), u, draft_probs=q, temperatures=torch.from_numpy(temps).cuda())
+    want = verify_oracle(logits, tokens, cu, u.cpu().numpy(), q, temps)
+    assert got[0].tolist() == want[0] and got[1].tolist() == want[1]
+    assert errors()[0] == 0
+
+
 def test_verify_greedy_takes_nan_as_the_maximum():
     logits, tokens, cu, u, _ = verify_case([1], 300, False, 4)
     logits[0, 77] = math.nan

@@ -367,7 +367,7 @@ class B200QuantizedBackend:
         tokens (any number, none too) or a tensor [B, k]. draft_probs: the draft's distribution at each drafted place,
         a list of tensors [k_i, V] or one [B, k, V]; None where the drafts are certain (copied from the prompt, or
         greedy). temperatures: a number or one per sequence (None = 1, 0 = greedy). uniforms fp32 [sum(k_i + 1)] in
-        [0, 1), drawn with ``generator`` where not given.
+        [0, 1), drawn with ``generator`` (of the backend's device) where not given.
 
         Returns (for every sequence its accepted drafts and the token that follows them, cache). The last of them is
         the next step's token, as after ``sample``."""
@@ -399,13 +399,13 @@ class B200QuantizedBackend:
             temps = None
             if temperatures is not None:
                 t = torch.as_tensor(temperatures, dtype=torch.float32).reshape(-1)
-                temps = t.expand(b).contiguous().to(dev) if t.numel() == 1 else t.to(dev)
+                temps = (t.expand(b) if t.numel() == 1 else t).contiguous().to(dev)
             if uniforms is None:
                 uniforms = torch.rand(R, device=dev, generator=generator)
                 if self.world_size > 1:
                     torch.distributed.broadcast(uniforms, torch.distributed.get_global_rank(self.group, 0)
                                                 if self.group is not None else 0, group=self.group)
-            uniforms = uniforms.to(device=dev, dtype=torch.float32)
+            uniforms = uniforms.to(device=dev, dtype=torch.float32).contiguous()
             before = self._grow(cache.tables, counts)
             try:
                 if cache.mirror is None or cache.mirror.arr.shape[0] < b:

@@ -185,6 +185,25 @@ def test_sampled_verification_follows_the_rule():
     assert [t.num_tokens for t in cache.tables] == [n + 1 + a for n, a in zip(lens, acc)]
 
 
+def test_verify_takes_strided_numbers_of_either_device():
+    shape = TINY["llama"]
+    model, _ = make_hf_model(shape, seed=4)
+    be = backend(model)
+    _, cache = be.prefill_ragged(prompts_of(shape["vocab"], [9, 20], seed=70))
+    start = [t.num_tokens for t in cache.tables]
+    u, temps = torch.rand((5, 3), generator=torch.Generator().manual_seed(2)), torch.tensor([[0.7, 9.0], [1.0, 9.0]])
+    answers = []
+    for dev in ("cpu", "cuda"):
+        for strided in (False, True):
+            uu, tt = (x.to(dev)[:, 0] for x in (u, temps))
+            if not strided:
+                uu, tt = uu.contiguous(), tt.contiguous()
+            got, cache = be.verify([1, 2], [[3, 9], [44]], cache, temperatures=tt, uniforms=uu)
+            answers.append(got)
+            be._shrink(cache.tables, start)
+    assert all(a == answers[0] for a in answers)
+
+
 def test_verify_failure_leaves_the_cache_as_it_was():
     shape = TINY["llama"]
     model, _ = make_hf_model(shape, seed=4)

@@ -450,7 +450,7 @@ __global__ void __launch_bounds__(RagCfg<D, Q8>::kThreads, 1)
   griddep_wait();
   const RagHead head = *reinterpret_cast<const RagHead*>(p.work);
   const bool planned = rag_made_for(head, p.max_rows, p.b, p.hq, p.hkv, p.max_blocks);
-  const int total = planned ? head.n_list * p.hkv : 0;  // (the merge records it: here that costs 0.3 us of each call)
+  const int total = planned ? head.n_list * p.hkv : 0;  // (the merge records it)
 
   if (warp >= 8) {
     regs_dec<C::kOtherRegs>();
@@ -998,8 +998,7 @@ __global__ void __launch_bounds__(RagCfg<D, Q8>::kThreads, 1)
           }
           if (!Q8 || k == lane >> 3) {
             l = a;
-            // (a maximum skips NaN, the sum does not: the state of a row that met one says so)
-            ml = l != l ? NAN : (m == -INFINITY ? -INFINITY : m * p.scale_log2);
+            ml = fmaf(l, 0.f, m * p.scale_log2);  // (a maximum skips NaN, the sum does not: NaN where the row met one)
           }
         }
         const bool both = wk.dual && wk.n1 > 0;  // two states of the same rows: the first warpgroup merges them
@@ -1035,8 +1034,8 @@ __global__ void __launch_bounds__(RagCfg<D, Q8>::kThreads, 1)
         tc_fence_after();
         if (warp_on) {
           float odd_sum = 0.f;  // a NaN once a value is one, or an infinity
-          // (every row sees a key: no sum at all means that all its scores were -inf, whose softmax is NaN)
-          const float inv = it.slot >= 0 ? 1.f : (l == 0.f ? NAN : 1.f / l);
+          // (every row sees a key: no sum at all means that all its scores were -inf; its output, 0 / 0, is NaN)
+          const float inv = it.slot >= 0 ? 1.f : 1.f / l;
           f0 *= inv;
           f1 *= inv;
           const int64_t slot_row = ((int64_t)it.slot * p.hkv + wk.head) * (2 * kRows) + (wk.dual ? 0 : w * kRows) + t;
@@ -1198,7 +1197,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32, kMergeCtas) ragged_merge_ker
         }
       }
       L = warp_sum(L);
-      const float inv = L == 0.f ? NAN : 1.f / L;  // (as in the attention)
+      const float inv = 1.f / L;  // (as in the attention: 0 / 0 where all scores are -inf)
       __nv_bfloat16* dst = p.out + (int64_t)(row0 + tok) * p.hq * D + ((int64_t)kvh * p.group + r % p.group) * D + lane * N;
       if constexpr (N == 4) {
         *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv));

@@ -370,7 +370,8 @@ class B200QuantizedBackend:
         [0, 1), drawn with ``generator`` (of the backend's device) where not given.
 
         Returns (for every sequence its accepted drafts and the token that follows them, cache). The last of them is
-        the next step's token, as after ``sample``."""
+        the next step's token, as after ``sample``. What the device cannot answer for one sequence (logits with a NaN, a
+        negative temperature) raises for the batch, and every table is as it was."""
         eng = self._need_model()
         if cache is None or not cache.tables:
             raise ValueError("verify needs the cache returned by prefill")

@@ -37,8 +37,10 @@ __device__ __forceinline__ bool rag_made_for(const RagHead& h, int64_t max_rows,
   return h.max_rows == max_rows && h.b == b && h.hq == hq && h.hkv == hkv && h.max_blocks == max_blocks;
 }
 
-// Splitting rule (see ragged_plan.cu): no list entry is longer than the work of one of `sms` equal shares, so an
-// item of n tiles gives ceil(n / share) entries and all of them together at most max_items + sms / hkv.
+// Splitting rule (see ragged_plan.cu): an item of n tiles gives at most ceil(n / share) entries, where share is at least
+// ceil(all tiles / max_merges) (and at least 2; it is lengthened where the entries then fit one wave). So fewer than
+// max_merges items are split, all items together give at most max_items + max_merges entries, and the split ones take
+// fewer than 2 * max_merges slots.
 static inline bool rag_shape(int64_t max_rows, int b, int hq, int hkv, int d, int sms, RagShape* s) {
   if (max_rows < 0 || max_rows > (1 << 26) || b < 0 || hq <= 0 || hkv <= 0 || hq % hkv || hq / hkv > 16) return false;
   if (d != 32 && d != 64 && d != 128) return false;

@@ -14,8 +14,8 @@
 //     memory (written over S) and V from the stage it was loaded to, taken as an MN-major operand, so that nothing is
 //     transposed. The two row tiles alternate: while one's softmax runs, the other's products do;
 //   * two warpgroups of softmax, one thread per row: no exchange between threads is needed for a row's maximum and
-//     sum. P is rounded to bf16, the type of V (one product has one operand type); the running maximum, the sum (of
-//     the unrounded values) and O are fp32. O is rescaled only when a row's maximum grew by more than 2^8 in the
+//     sum. P is rounded to bf16, the type of V (one product has one operand type), over an int8 cache P times the
+//     value's scale (the codes are exact in bf16); the running maximum, the sum (of the unrounded values) and O are fp32. O is rescaled only when a row's maximum grew by more than 2^8 in the
 //     exponentials' scale: until then exponentials up to 2^8 stay far inside the range of fp32 and bf16, and the
 //     final division by the sum removes the common factor.
 // A CTA takes several items, dealt out by length, and its K/V and Q loads run ahead into the next one. An item of one row
@@ -27,19 +27,22 @@
 // there, and 0 * V must be zero too: rows of V behind the item's last key are zeroed in the stage. What an infinity or a
 // NaN in the V of a masked key would leave in the output shows there as one: a piece of work whose output holds any is
 // done over in a second pass, which looks over the V rows that some row may not see, and in a tile with such a value
-// leaves the product to the softmax threads, over the keys each row sees.
+// leaves the product to the softmax threads, over the keys each row sees. A NaN that a row does see (in its query, in K or V)
+// makes its output NaN, and so does a row of nothing but -inf.
 //
 // What bounds it, on a B200 (24/8 heads of 128 unless said; floors at 6.55 TB/s and 1675 TFLOP/s):
-//   * an 8192-token prompt, 380-450 us with the clock, 0.92-1.1 PFLOP/s, floor 246: a row tile takes its softmax (2.0 k
+//   * an 8192-token prompt, 430 us (380-450 with the clock), 0.96 PFLOP/s, floor 246: a row tile takes its softmax (2.0 k
 //     cycles, two warpgroups sharing an SM's exponentials) and then its own two products (1.0 k); the two row tiles
 //     overlap to 3.2 k cycles, of which the products of both fill two thirds. Tried and slower: the products of each row
 //     tile from a warp of its own (they interleave, and both softmaxes wait for both; a fifth), steps of 64 keys with two
 //     score buffers (a third), reading the scores from tensor memory twice instead of holding 128 of them (up to a
 //     tenth). A part of the exponentials as polynomials, and the rescaling of O behind them, gained nothing;
-//   * 32 requests of 5 tokens over 300 to 4000 cached ones, 57 us, floor 35: the longest CTA's share is 1.2 times the mean,
+//   * 32 requests of 5 tokens over 300 to 4000 cached ones, 58 us, floor 35: the longest CTA's share is 1.2 times the mean,
 //     and the merge adds 5 (60 with all loads from one warp, whose 2 KB copies do not start fast enough);
+//   * one token over 32763, 37 us, floor 21: 8 tiles a CTA, so that the start, the first loads and the merge weigh as much;
 //   * 24 packed prompts of 18 to 2005 tokens, 14/2 heads of 64, 65 us: the exponentials of whole 128 x 128 tiles, most of
-//     them cut by the diagonal; the products would take 13;
+//     them cut by the diagonal (their pipe is busy 44 % of the time); the products would take 13. (128 columns of tensor
+//     memory are not used at this head size; the figures above for other ways were taken at heads of 128.)
 //   * 16 chunks over up to 3800 cached tokens, bf16, 59 us: two or three short items a CTA, each with an end of its own;
 //     int8, 82: codes to bf16 by one warpgroup (2.0 k cycles a tile) and a softmax of 4.2 k cycles, the scales'
 //     products included, in code that strains the instruction caches (95 while all of it was unrolled, with a row per

@@ -15,9 +15,15 @@
 // shared memory, whose eight CTAs of 128 KB find room a third at a time. The draw's sums are in 64 bits: with 10^5 entries
 // the running sum's steps are so close that 32-bit sums put the drawn index one off in about one of a hundred draws,
 // where 64-bit sums of 64-bit exponentials do in none.
-// 48 requests of 1 to 8 drafts, 128256 entries, draft probabilities (162 MB, 25 us at 6.55 TB/s): 85 us. By
-// themselves the rows' states take 32, the decision 33 and the rest 30 (they overlap in part): the latter two are a chain of
-// dependent loads, then 64-bit exponentials.
+// The test of a draft holds p(d) against the 32-bit sum of the row's state: approximate exponentials of arguments up to 20
+// or so that matter (2^-18.5 relative at the most, three roundings of the argument) and a sum of 32 terms a thread, then of
+// threads and chunks (2^-19). A draft whose u q(d) lies closer to p(d) than 2^-17 of it may fall either way: at most one of
+// 65 thousand drafts.
+// 48 requests of 1 to 8 drafts, 128256 entries, draft probabilities (162 MB, 25 us at 6.55 TB/s): 82 us. By
+// themselves the rows' states take 34, the decision 34 and the rest 31 (they overlap in part): the latter two issue in half of
+// their cycles, with the 64-bit pipe at a quarter of its rate and the memory at a tenth: 64-bit exponentials, each a long chain
+// of instructions, on every entry of the stopping row. One request of 4 drafts, 50257 entries: 17 us, of which the decision is
+// 15 on 16 CTAs: barriers and dependent loads, each CTA reading all of the request's states before its segment.
 #include "common.cuh"
 
 namespace {

@@ -1024,6 +1024,9 @@ __global__ void __launch_bounds__(RagCfg<D, Q8>::kThreads, 1)
         }
         ok = bar_wait(&ofull[w], co++ & 1, 522);
         float f0 = 1.f, f1 = 0.f;
+        // a state whose row saw no key there is left out of a merge, whatever its output holds; one whose weight is merely
+        // nothing in 32 bits is not, for an infinity or NaN in it counts
+        bool out0 = false, out1 = true;
         if (both) {
           ok = ok && bar_wait(mlready, duals++ & 1, 529);
           const float2 o1 = mls[t];
@@ -1031,6 +1034,8 @@ __global__ void __launch_bounds__(RagCfg<D, Q8>::kThreads, 1)
           f0 = ml == -INFINITY ? 0.f : exp2f(ml - top);
           f1 = o1.x == -INFINITY ? 0.f : exp2f(o1.x - top);
           l = (f0 == 0.f ? 0.f : f0 * l) + (f1 == 0.f ? 0.f : f1 * o1.y);
+          out0 = ml == -INFINITY && top != -INFINITY;
+          out1 = o1.x == -INFINITY && top != -INFINITY;
           ml = top;
         }
         if (!ok) break;
@@ -1049,14 +1054,14 @@ __global__ void __launch_bounds__(RagCfg<D, Q8>::kThreads, 1)
             tmem_ld32(to + c, o);
             tc_wait_ld();
 #pragma unroll
-            for (int x = 0; x < 32; ++x) o[x] = f0 == 0.f ? 0u : __float_as_uint(__uint_as_float(o[x]) * f0);
+            for (int x = 0; x < 32; ++x) o[x] = out0 ? 0u : __float_as_uint(__uint_as_float(o[x]) * f0);
             if (both) {
               uint32_t o1[32];
               tmem_ld32(to + D + c, o1);
               tc_wait_ld();
 #pragma unroll
               for (int x = 0; x < 32; ++x)
-                if (f1 != 0.f) o[x] = __float_as_uint(fmaf(__uint_as_float(o1[x]), f1, __uint_as_float(o[x])));
+                if (!out1) o[x] = __float_as_uint(fmaf(__uint_as_float(o1[x]), f1, __uint_as_float(o[x])));
             }
             if constexpr (!Q8) {
 #pragma unroll
@@ -1182,18 +1187,20 @@ __global__ void __launch_bounds__(kMergeWarps * 32, kMergeCtas) ragged_merge_ker
       for (int s = lane + 32; s < parts; s += 32) M = fmaxf(M, p.ws_ml[first + s * step].x);
       M = warp_max(M);
       float L = 0.f, f = 0.f, o[N] = {};
+      unsigned held = 0;  // the parts that hold a key of the row (the outputs of the others are left out, whatever they are)
 #pragma unroll 1
       for (int s = 0; s < parts; s += kMergeBatch) {
         if ((s & 31) == 0) {
           if (s > 0) ml = s + lane < parts ? p.ws_ml[first + (s + lane) * step] : make_float2(-INFINITY, 0.f);
           f = ml.x == -INFINITY ? 0.f : exp2f(ml.x - M);
           L += f == 0.f ? 0.f : f * ml.y;
+          held = __ballot_sync(0xffffffffu, ml.x != -INFINITY);
         }
         if (s > 0) fetch(s);
 #pragma unroll
         for (int y = 0; y < kMergeBatch; ++y) {
           const float fy = __shfl_sync(0xffffffffu, f, (s + y) & 31);
-          if (s + y < parts && fy != 0.f) {
+          if (held >> ((s + y) & 31) & 1u) {
 #pragma unroll
             for (int x = 0; x < N; ++x) o[x] = fmaf(fy, reinterpret_cast<const float*>(&v[y])[x], o[x]);
           }

@@ -608,6 +608,35 @@ def test_attention_gives_nan_where_every_score_is_minus_infinity(q, ctx):
     assert errors()[0] == 0
 
 
+@pytest.mark.parametrize("kv8", [False, True])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("q,ctx,big,at", [([1], [255], 3, 200), ([1], [255], 200, 3), ([1], [20000], 5, 15000), ([1], [20000], 15000, 5),
+                                          ([200], [9000], 7, 6000), ([60], [0], 3, 20), ([120], [0], 3, 50)])
+def test_attention_keeps_a_value_whose_weight_is_zero_in_32_bits(q, ctx, big, at, bad, kv8):
+    """One key takes all the weight; another, in a tile or part of its own, holds an infinity or NaN in V: zero times it is NaN, as
+    in the plain form, although the part's whole weight is zero when states are merged."""
+    hq, hkv, d = 24, 8, 128
+    c = Case(q, ctx, hq, hkv, d, kv8, seed=4).fill()
+    place = lambda p: (c.tables[0, p // 16], 2, p % 16)
+    c.q[:] = 1.0
+    c.k.zero_()
+    if kv8:  # 16 in every place: 181 above the other scores
+        c.k[place(big)] = 127
+        c.sc["k_scales"][place(big)] = 16.0 / 127
+        c.sc["v_scales"][place(at)] = bad
+    else:
+        c.k[place(big)] = 16.0
+        c.v[place(at)][5] = bad
+    out = c.run().view(-1, hq, d)
+    assert errors()[0] == 0
+    first = max(0, at - ctx[0])  # the first new token that sees it
+    cols = slice(None) if kv8 else slice(5, 6)
+    assert not torch.isfinite(out[first:, 6:9, cols]).any()
+    rest = torch.ones_like(out, dtype=torch.bool)
+    rest[first:, 6:9, cols] = False
+    assert torch.isfinite(out[rest]).all()
+
+
 def test_attention_matches_the_decode_kernel():
     """Single tokens: the operator gives what paged_decode_attn gives (which rounds q * scale to bf16)."""
     c = Case([1] * 6, [3, 63, 500, 1999, 0, 128], 24, 8, 128, seed=8).fill()

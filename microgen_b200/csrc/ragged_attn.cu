@@ -1036,7 +1036,7 @@ __global__ void __launch_bounds__(RagCfg<D, Q8>::kThreads, 1)
           l = (f0 == 0.f ? 0.f : f0 * l) + (f1 == 0.f ? 0.f : f1 * o1.y);
           out0 = ml == -INFINITY && top != -INFINITY;
           out1 = o1.x == -INFINITY && top != -INFINITY;
-          ml = top;
+          ml = fmaf(l, 0.f, top);  // (NaN beside an empty state too: fmaxf has skipped it)
         }
         if (!ok) break;
         tc_fence_after();

@@ -637,6 +637,29 @@ def test_attention_keeps_a_value_whose_weight_is_zero_in_32_bits(q, ctx, big, at
     assert torch.isfinite(out[rest]).all()
 
 
+@pytest.mark.parametrize("kv8", [False, True])
+@pytest.mark.parametrize("q,ctx,hq,hkv,d,req,at", [([244, 296, 69], [49, 102, 142], 8, 8, 128, 1, 287), ([40], [630], 12, 12, 64, 0, 592),
+                                                   ([34, 37], [150, 625], 12, 12, 64, 1, 607)])
+def test_attention_keeps_a_nan_in_a_part_whose_last_tile_a_row_does_not_see(q, ctx, hq, hkv, d, req, at, kv8):
+    """A part of a split item ends in a tile that lies behind some of its rows, and the tile before holds a NaN in K: the part's
+    two states are a NaN and an empty one, and the merge of the parts must not take what comes of them for empty."""
+    c = Case(q, ctx, hq, hkv, d, kv8, seed=5).fill()
+    assert work_list(c.plan)[1].shape[0] > 0  # the plan splits these
+    want, mag = c.oracle()
+    place = (c.tables[req, at // 16], 1, at % 16)
+    if kv8:
+        c.sc["k_scales"][place] = math.nan
+    else:
+        c.k[place][0] = math.nan
+    bad = torch.zeros(want.shape[:2], dtype=torch.bool, device="cuda")
+    start = sum(q[:req])
+    bad[start + max(0, at - ctx[req]):start + q[req], hq // hkv:2 * (hq // hkv)] = True
+    got = c.run().double().view_as(want)
+    assert torch.isnan(got[bad]).all()
+    assert ((got - want).abs() <= 2.0 ** -7 * 1.05 * mag + 1e-6)[~bad].all()
+    assert errors()[0] == 0
+
+
 def test_attention_matches_the_decode_kernel():
     """Single tokens: the operator gives what paged_decode_attn gives (which rounds q * scale to bf16)."""
     c = Case([1] * 6, [3, 63, 500, 1999, 0, 128], 24, 8, 128, seed=8).fill()

@@ -44,7 +44,7 @@
 //     them cut by the diagonal (their pipe is busy 44 % of the time); the products would take 13. (128 columns of tensor
 //     memory are not used at this head size; the figures above for other ways were taken at heads of 128.)
 //   * 16 chunks over up to 3800 cached tokens, bf16, 59 us: two or three short items a CTA, each with an end of its own;
-//     int8, 82: codes to bf16 by one warpgroup (2.0 k cycles a tile) and a softmax of 4.2 k cycles, the scales'
+//     int8, 83: codes to bf16 by one warpgroup (2.0 k cycles a tile) and a softmax of 4.2 k cycles, the scales'
 //     products included, in code that strains the instruction caches (95 while all of it was unrolled, with a row per
 //     thread).
 #include <type_traits>
